@@ -151,6 +151,7 @@ const char* fnet_strerror(int code) {
         case FNET_E_HIP: return "HIP runtime error (see fnet_last_hip_error)";
         case FNET_E_UNSUPPORTED: return "unsupported configuration";
         case FNET_E_TOO_LARGE: return "input larger than the stated maximum of this allocation-free entry point -- nothing was launched";
+        case FNET_E_OVERLAP: return "two tensors of a list that is written share memory -- nothing was launched";
         default: return "unknown error";
     }
 }

@@ -1,0 +1,118 @@
+// Vector access at any alignment and lane reductions for the row / list kernels (fnet_block_norm*.hip, fnet_tensor_list.hip).
+#pragma once
+#include <hip/hip_fp16.h>
+
+#include "fnet_common.h"
+
+// 16 bytes at a time whatever the address: rows of an odd width and gradients packed into one bucket start at any multiple of the element
+// size.  The global memory path of gfx950 takes such addresses (the HSA target runs in unaligned-access mode), and with the element's own
+// alignment declared here the compiler still emits one global_load_dwordx4 / global_store_dwordx4, so there is one code path for aligned
+// and unaligned operands.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
+typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
+
+// An address that came as an integer, as a pointer to global memory: without the named address space every access through it would be a
+// flat one, which also occupies the LDS counter.
+template <typename T>
+__device__ __forceinline__ T* gptr(uint64_t a) {
+    return (T*)(__attribute__((address_space(1))) T*)a;
+}
+
+struct f16_t { uint16_t b; };      // raw fp16 bits (bf16_t is a plain uint16_t: the two must be different types)
+
+template <typename T> struct VecOf;
+template <> struct VecOf<float> { static constexpr int V = 4; typedef u32x4_a4 vec; };
+template <> struct VecOf<bf16_t> { static constexpr int V = 8; typedef u32x4_a2 vec; };
+template <> struct VecOf<f16_t> { static constexpr int V = 8; typedef u32x4_a2 vec; };
+
+template <typename T> __device__ __forceinline__ float elem_to_f(T v);
+template <> __device__ __forceinline__ float elem_to_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ float elem_to_f<bf16_t>(bf16_t v) { return bf2f(v); }
+template <> __device__ __forceinline__ float elem_to_f<f16_t>(f16_t v) { return (float)__builtin_bit_cast(_Float16, v.b); }
+template <typename T> __device__ __forceinline__ T f_to_elem(float v);          // round to nearest even
+template <> __device__ __forceinline__ float f_to_elem<float>(float v) { return v; }
+template <> __device__ __forceinline__ bf16_t f_to_elem<bf16_t>(float v) { return f2bf(v); }
+template <> __device__ __forceinline__ f16_t f_to_elem<f16_t>(float v) { return f16_t{__builtin_bit_cast(uint16_t, (_Float16)v)}; }
+
+// the 16 bytes as loaded -> V floats, and back
+template <typename T> __device__ __forceinline__ void unpack16(const u32x4& w, float* v);
+template <> __device__ __forceinline__ void unpack16<float>(const u32x4& w, float* v) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = __uint_as_float(w[k]);
+}
+template <> __device__ __forceinline__ void unpack16<bf16_t>(const u32x4& w, float* v) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        v[2 * k] = __uint_as_float(w[k] << 16);
+        v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+    }
+}
+template <> __device__ __forceinline__ void unpack16<f16_t>(const u32x4& w, float* v) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        v[2 * k] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[k] & 0xffffu));
+        v[2 * k + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[k] >> 16));
+    }
+}
+template <typename T> __device__ __forceinline__ u32x4 pack16(const float* v);
+template <> __device__ __forceinline__ u32x4 pack16<float>(const float* v) {
+    return (u32x4){__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+}
+template <> __device__ __forceinline__ u32x4 pack16<bf16_t>(const float* v) {
+    return (u32x4){f2bf_pk(v[0], v[1]), f2bf_pk(v[2], v[3]), f2bf_pk(v[4], v[5]), f2bf_pk(v[6], v[7])};
+}
+template <> __device__ __forceinline__ u32x4 pack16<f16_t>(const float* v) {
+    u32x4 w;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        w[k] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * k]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * k + 1]) << 16);
+    return w;
+}
+
+// n (1 .. V) leading elements of the 16-byte chunk at p; the rest reads as zero / is left alone
+template <typename T>
+__device__ __forceinline__ void load_chunk(const T* p, int n, float* v) {
+    constexpr int V = VecOf<T>::V;
+    if (n >= V) {
+        const u32x4 w = *reinterpret_cast<const typename VecOf<T>::vec*>(p);
+        unpack16<T>(w, v);
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = k < n ? elem_to_f<T>(p[k]) : 0.f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store_chunk(T* p, int n, const float* v) {
+    constexpr int V = VecOf<T>::V;
+    if (n >= V) {
+        *reinterpret_cast<typename VecOf<T>::vec*>(p) = pack16<T>(v);
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+            if (k < n) p[k] = f_to_elem<T>(v[k]);
+    }
+}
+
+// Sum over groups of L consecutive lanes (L = 8 .. 64, a power of two), the result in every lane of the group.  Inside 16 lanes by DPP:
+// quad_perm exchanges neighbours and pairs, and once a group of four (eight) holds one value the half mirror (mirror) exchanges groups.
+template <int CTRL>
+__device__ __forceinline__ float dpp_f(float v) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+template <int L>
+__device__ __forceinline__ float lane_sum(float v) {
+    v += dpp_f<0xB1>(v);                 // quad_perm [1,0,3,2]
+    v += dpp_f<0x4E>(v);                 // quad_perm [2,3,0,1]
+    if (L >= 8) v += dpp_f<0x141>(v);    // row_half_mirror
+    if (L >= 16) v += dpp_f<0x140>(v);   // row_mirror
+    if (L >= 32) v += __shfl_xor(v, 16, 64);
+    if (L >= 64) v += __shfl_xor(v, 32, 64);
+    return v;
+}
+
+#define DISPATCH_T3(dtype, ...)                                      \
+    if ((dtype) == FNET_BF16) { using T = bf16_t; __VA_ARGS__; }      \
+    else if ((dtype) == FNET_F32) { using T = float; __VA_ARGS__; }   \
+    else if ((dtype) == FNET_F16) { using T = f16_t; __VA_ARGS__; }   \
+    else return FNET_E_BADARG;

@@ -15,7 +15,7 @@ LIB_PATH = os.environ.get("FNET_LIB") or os.path.join(os.path.dirname(_HERE), "l
 OP_DTYPE = np.dtype([("op", "<i4"), ("dtype", "<i4"), ("i", "<i4", (30,)), ("f", "<f4", (8,)), ("p", "<u8", (10,))], align=True)
 assert OP_DTYPE.itemsize == 240, OP_DTYPE.itemsize
 
-F32, BF16 = 0, 1
+F32, BF16, F16 = 0, 1, 2      # F16: block norms and tensor lists only
 PAD = {"zeros": 0, "replicate": 1, "reflect": 2, "circular": 3}
 ACT = {"relu": 0, "leaky_relu": 1, "gelu": 2, "silu": 3, "identity": 4}
 OUTACT = {"linear_clamp": 0, "sigmoid_tanh": 1}
@@ -94,6 +94,17 @@ def lib() -> ctypes.CDLL:
     for name, args in sigs.items():
         getattr(L, name).restype = ctypes.c_int
         getattr(L, name).argtypes = args
+    u64p, i64p, i32p, f64 = vp, vp, vp, ctypes.c_double          # host arrays, passed by address
+    sigs = {"fnet_block_norm_fwd": [ctypes.c_char_p, vp], "fnet_block_norm_bwd": [ctypes.c_char_p, vp],
+            "fnet_block_norm_workspace": [ctypes.c_char_p, ctypes.POINTER(i64)],
+            "fnet_list_norm_partials": [i32, u64p, i64p, i32p, i32, vp, i32, vp, i32, ctypes.POINTER(i32), vp, f64, f64, vp],
+            "fnet_list_clock": [vp, f64, f64, vp],
+            "fnet_list_norm_finish": [vp, i32, i32, vp, vp],
+            "fnet_list_scale": [i32, u64p, i64p, i32p, i32, vp, vp, i32, i32, vp, f64, vp, vp],
+            "fnet_list_adam": [i32, u64p, u64p, u64p, u64p, u64p, i64p, i32p, ctypes.c_char_p, vp]}
+    for name, args in sigs.items():
+        getattr(L, name).restype = ctypes.c_int
+        getattr(L, name).argtypes = args
     L.fnet_set_knob.restype = ctypes.c_int
     L.fnet_set_knob.argtypes = [ctypes.c_char_p, ctypes.c_int32]
     if L.fnet_abi_version() != ABI_VERSION:
@@ -107,7 +118,9 @@ EXPORTS = ["fnet_abi_version", "fnet_strerror", "fnet_last_hip_error", "fnet_dev
            "fnet_graph_launch", "fnet_graph_destroy", "fnet_spatial_gradients", "fnet_divergence", "fnet_timer_create",
            "fnet_timer_start", "fnet_timer_stop", "fnet_timer_elapsed_ms", "fnet_timer_destroy", "fnet_unet_param_count",
            "fnet_rollout_create", "fnet_rollout_set_weights", "fnet_rollout_set_masks", "fnet_rollout_set_state", "fnet_rollout_add_impulse",
-           "fnet_rollout_step", "fnet_rollout_state_ptr", "fnet_rollout_read_state", "fnet_rollout_destroy"]
+           "fnet_rollout_step", "fnet_rollout_state_ptr", "fnet_rollout_read_state", "fnet_rollout_destroy",
+           "fnet_block_norm_fwd", "fnet_block_norm_bwd", "fnet_block_norm_workspace", "fnet_list_norm_partials", "fnet_list_clock", "fnet_list_norm_finish",
+           "fnet_list_scale", "fnet_list_adam"]
 
 
 def check(rc: int, what: str = "", ops: Optional[np.ndarray] = None, failed: int = -1) -> None:
@@ -127,6 +140,19 @@ def check(rc: int, what: str = "", ops: Optional[np.ndarray] = None, failed: int
 def current_stream_ptr() -> int:
     import torch
     return int(torch.cuda.current_stream().cuda_stream)
+
+
+def call_on(t, name: str, *args) -> None:
+    """An entry point whose last argument is the stream, on the current stream of the device that tensor `t` lies on."""
+    import torch
+    fn, dev = getattr(lib(), name), t.device
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        check(rc, name)
 
 
 def run_ops(ops: np.ndarray, stream: Optional[int] = None) -> None:

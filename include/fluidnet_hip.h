@@ -36,10 +36,12 @@ extern "C" {
 #define FNET_E_HIP (-2)      /* a HIP runtime call failed; fnet_last_hip_error() has the code */
 #define FNET_E_UNSUPPORTED (-3)
 #define FNET_E_TOO_LARGE (-4)  /* the input exceeds the stated maximum of an allocation-free entry point (nothing launched) */
+#define FNET_E_OVERLAP (-5)    /* two tensors of a list that is written share memory (nothing launched) */
 
 /* element type of P-tensors */
 #define FNET_F32 0
 #define FNET_BF16 1
+#define FNET_F16 2            /* block norms and tensor lists only */
 
 /* padding mode (ml/models/unet.py:13 PaddingType; ml/training/physics_loss.py:32-33) */
 #define FNET_PAD_ZEROS 0
@@ -262,6 +264,96 @@ int fnet_rollout_step(void* handle, int32_t frames, void* stream);
 int fnet_rollout_state_ptr(void* handle, float** device_state, float** device_prev_density);
 int fnet_rollout_read_state(void* handle, float* host_state, void* stream);
 int fnet_rollout_destroy(void* handle);
+
+/*
+ * Norms around a residual block, with its gate and residual scale, over the last axis of row-major operands (a row = one token, or one
+ * pixel of a channels-last image).  No reference counterpart (its blocks normalise over pixels, ml/models/unet.py:17-28); the host
+ * mirror is fluidnet_amd/models/block_norm.py.
+ *   N(v) = v / sqrt(mean v^2 + eps)  or  (v - mean) / sqrt(var + eps)
+ *   u = POST ? N(branch) * post_weight + post_bias : branch
+ *   y = x + residual_scale * scale[c] * act(gate) * u           (branch == 0: y = x, nothing written)
+ *   h = N(y) * pre_weight + pre_bias                            (h == 0: not computed; y is taken before it is rounded)
+ * Row r of an operand starts at r * its row stride (elements); the elements of a row are adjacent.  y, h, dx, dbranch and an elementwise
+ * dgate are dense.  Any alignment of the element size.  Absent pointers are 0 (an absent weight is 1, an absent bias 0).  Statistics, sums
+ * and products are 32-bit; sums over rows are taken in a fixed order.
+ * Backward recomputes y from x, branch and gate, and reads the forward's stats.  Gradients whose pointer is 0 are not computed.
+ */
+#define FNET_NORM_RMS 0
+#define FNET_NORM_LAYER 1
+#define FNET_GATE_NONE 0
+#define FNET_GATE_ELEMENT 1   /* a value per element */
+#define FNET_GATE_TOKEN 2     /* a value per row */
+#define FNET_GATE_SAMPLE 3    /* a row of values per `tokens` consecutive rows */
+#define FNET_GATE_CHANNEL 4   /* one row of values for all rows */
+#define FNET_GATE_IDENTITY 0
+#define FNET_GATE_SIGMOID 1
+#define FNET_GATE_TANH 2
+#define FNET_BLOCK_NORM_MAX_WIDTH 16384
+typedef struct FnetBlockNorm {
+    int64_t rows;             /* < 2^31 */
+    int64_t tokens;           /* rows per sample (FNET_GATE_SAMPLE; divides rows) */
+    int64_t x_stride, branch_stride, gate_stride, dy_stride, dh_stride;   /* row strides; gate_stride: of a row / sample of the gate */
+    int32_t width;            /* 1 .. FNET_BLOCK_NORM_MAX_WIDTH */
+    int32_t dtype;            /* x, branch, y, h and their gradients */
+    int32_t param_dtype;      /* weights, biases, scale and their gradients: FNET_F32 or dtype */
+    int32_t gate_dtype;       /* gate and its gradient: FNET_F32 or dtype */
+    int32_t kind, post;       /* FNET_NORM_*; 1: the branch is normalised */
+    int32_t gate_kind, gate_act;
+    float residual_scale, eps;
+    uint64_t x, branch, gate, scale, post_weight, post_bias, pre_weight, pre_bias;
+    uint64_t y, h;            /* forward results */
+    uint64_t stats;           /* float [4][rows]: mean and 1/deviation of the branch, then of y; 0: not kept (forward only) */
+    uint64_t dy, dh;          /* 0: zero */
+    uint64_t dx, dbranch, dgate, dscale, dpost_weight, dpost_bias, dpre_weight, dpre_bias;
+    uint64_t workspace;       /* backward: fnet_block_norm_workspace bytes, 16-byte aligned */
+    int64_t workspace_bytes;
+} FnetBlockNorm;
+int fnet_block_norm_fwd(const FnetBlockNorm* host_args, void* stream);
+int fnet_block_norm_bwd(const FnetBlockNorm* host_args, void* stream);
+/* bytes of workspace that fnet_block_norm_bwd needs for these arguments (0 if none); host only */
+int fnet_block_norm_workspace(const FnetBlockNorm* host_args, int64_t* bytes);
+
+/*
+ * Lists of tensors: the global gradient norm, clipping in place and a clipped Adam step, for any number of separate tensors of the three
+ * element types (ml/training/trainer.py:190-195; FNET_OP_GRAD_NORM / FNET_OP_ADAM are the same for one flat fp32 buffer).  The list
+ * is given by host arrays of device addresses, element counts and types, read during the call and passed on as kernel arguments; a dense
+ * tensor of any layout is its memory in order.  Entries of no elements are skipped.  All of it is capturable.
+ *   fnet_list_norm_partials  sums of squares / of absolutes / maxima of the list's parts in 64 bits, *n_partials of them (at most `capacity`,
+ *                            which 2048 + n / 64 + 256 * n_strided + 8 always covers); `clock`, if not 0, is advanced as one Adam step
+ *   fnet_list_clock          advances clock = (t, beta1^t, beta2^t) alone (a step without clipping)
+ *   fnet_list_norm_finish    the norm itself from the partials
+ *   fnet_list_scale          g *= min(1, max_norm / (norm + 1e-6)), the norm taken from the partials, or from *norm if those are 0; the
+ *                            norm is also stored to *norm_out if that is not 0.  FNET_E_OVERLAP if two dense tensors share memory
+ *   fnet_list_adam           one step; parameters that are not fp32 have an fp32 master that is updated and of which they are the rounding
+ */
+#define FNET_LIST_MAXDIM 6
+#define FNET_LIST_NORM_2 0
+#define FNET_LIST_NORM_1 1
+#define FNET_LIST_NORM_INF 2
+typedef struct FnetStridedTensor {    /* a tensor that is no dense block: sizes and strides (elements, positive, no overlap) */
+    uint64_t ptr;
+    int32_t dtype, ndim;
+    int64_t size[FNET_LIST_MAXDIM], stride[FNET_LIST_MAXDIM];
+} FnetStridedTensor;
+typedef struct FnetAdamList {
+    double lr, beta1, beta2, eps, weight_decay;
+    double max_norm;          /* < 0: no clipping */
+    const double* partials;   /* device: from fnet_list_norm_partials over the gradients (2-norm) */
+    const double* clock;      /* device: t, beta1^t, beta2^t of this step (already advanced) */
+    const double* lr_device;  /* device, or 0: lr */
+    float* norm_out;          /* device, or 0: the norm before clipping */
+    int32_t n_partials;
+} FnetAdamList;
+int fnet_list_norm_partials(int32_t n, const uint64_t* host_ptr, const int64_t* host_numel, const int32_t* host_dtype, int32_t n_strided,
+                            const FnetStridedTensor* host_strided, int32_t norm_kind, double* partials, int32_t capacity,
+                            int32_t* n_partials, double* clock, double beta1, double beta2, void* stream);
+int fnet_list_clock(double* clock, double beta1, double beta2, void* stream);
+int fnet_list_norm_finish(const double* partials, int32_t n_partials, int32_t norm_kind, float* norm_out, void* stream);
+int fnet_list_scale(int32_t n, const uint64_t* host_ptr, const int64_t* host_numel, const int32_t* host_dtype, int32_t n_strided,
+                    const FnetStridedTensor* host_strided, const double* partials, int32_t n_partials, int32_t norm_kind, const float* norm,
+                    double max_norm, float* norm_out, void* stream);
+int fnet_list_adam(int32_t n, const uint64_t* host_param, const uint64_t* host_grad, const uint64_t* host_exp_avg, const uint64_t* host_exp_avg_sq,
+                   const uint64_t* host_master, const int64_t* host_numel, const int32_t* host_dtype, const FnetAdamList* host_args, void* stream);
 
 #ifdef __cplusplus
 }
