@@ -10,7 +10,9 @@ Two execution engines for the optimisation step of train_epoch (trainer.py:142-2
       (fluidnet_amd.engine.train_plan.RolloutTrainPlan) replayed per batch with no host sync; batches whose shape has no
       plan yet build one (at most `max_plans` shapes, e.g. the ragged last batch), others fall back to the autograd engine.
   engine="autograd": the literal loop of the reference (_compute_rollout_loss + loss.backward()) through the
-      torch.autograd wrappers of fluidnet_amd.UNet / PhysicsAwareLoss, followed by FusedClipAdam.
+      torch.autograd wrappers of fluidnet_amd.UNet / PhysicsAwareLoss, followed by FusedClipAdam.  This engine also trains any
+      other module that maps [B,6,H,W] to [B,3,H,W] (for instance one with the norms of models/block_norm.py): its separate
+      parameters, of any of the three element types, are clipped and stepped by ClipAdam.
 Both give the loss dict keys of the reference (mse, divergence, gradient, emitter, total).
 Not carried over: MLflow logging, matplotlib plots, GradScaler (bf16 needs none), the torchmetrics-based validation
 metrics -- validate() returns the averaged loss terms only.
@@ -20,23 +22,24 @@ fluidnet_amd/training/dp.py.
 from __future__ import annotations
 
 import time
+from inspect import getattr_static
 from pathlib import Path
-from typing import Any, Dict, Optional, Tuple
+from typing import Any, Dict, Optional, Tuple, Union
 
 import torch
 
 from ..engine.train_plan import RolloutTrainPlan
 from .dp import dp_train_step, torch_all_reduce
 from .early_stopping import EarlyStopping
-from .optim import FusedClipAdam
+from .optim import ClipAdam, FusedClipAdam
 from .physics_loss import PhysicsAwareLoss
 from .metrics import MetricsTracker, validation_metrics
 
 
 class _Scheduler:
-    """plateau / cosine / step learning-rate schedules with torch's semantics, acting on FusedClipAdam.param_groups."""
+    """plateau / cosine / step learning-rate schedules with torch's semantics, acting on the optimizer's param_groups."""
 
-    def __init__(self, opt: FusedClipAdam, cfg) -> None:
+    def __init__(self, opt: Union[FusedClipAdam, ClipAdam], cfg) -> None:
         import math
         self.opt, self.cfg, self.kind = opt, cfg, cfg.lr_scheduler_type
         if self.kind not in ("plateau", "cosine", "step"):
@@ -93,7 +96,13 @@ class Trainer:
             emitter_weight=pl.emitter_weight, grid_spacing=pl.grid_spacing, enable_divergence=pl.enable_divergence,
             enable_gradient=pl.enable_gradient, enable_emitter=pl.enable_emitter, padding_mode=config.padding_mode,
             stencil_mode=pl.stencil_mode)
-        self.optimizer = FusedClipAdam(model, config.learning_rate, config.gradient_clip_norm if config.gradient_clip_enabled else None)
+        clip = config.gradient_clip_norm if config.gradient_clip_enabled else None
+        if getattr_static(model, "flat_params", None) is not None:
+            self.optimizer = FusedClipAdam(model, config.learning_rate, clip)
+        elif engine == "plan":
+            raise ValueError("engine='plan' runs fluidnet_amd.UNet; other modules train with engine='autograd'")
+        else:                                                # separate parameters
+            self.optimizer = ClipAdam([p for p in model.parameters() if p.requires_grad], config.learning_rate, clip)
         self.scaler = None                                   # bf16 storage / fp32 accumulate needs no loss scaling
         self.scheduler = _Scheduler(self.optimizer, config) if config.use_lr_scheduler else None
         if getattr(config, "variant", None):                 # curriculum runs: <checkpoints>/<relative dir>/<arch>_<variant> (trainer.py:71-74)
