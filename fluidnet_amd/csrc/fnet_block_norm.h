@@ -1,62 +1,115 @@
-// Shared by the forward and the backward of the norms around a residual block (fnet_block_norm.hip, fnet_block_norm_bwd.hip).
+// Shared by the forward and the backward of the norms around a residual block (fnet_block_norm*.hip).
 #pragma once
 #include "fnet_vec.h"
 
-// How rows lie on lanes.  A row belongs to L lanes (8 .. 1024) that hold it in registers from its one load to its last store, E elements
-// each, in chunks of 16 bytes: lane l of a row holds chunks l, l + L, ...  Up to 64 lanes a row lies inside a wave (DPP sums, no barrier,
-// 256 / L rows per block at a time); above that a block is one row.
+// How rows lie on lanes.  A row is held in registers from its one load to its last store, E elements a lane in chunks of 16 bytes: lane l of
+// a row holds chunks l, l + lanes, ...
+//   L = 8 .. 64  that many lanes of one wave: sums stay inside the wave, no barrier, 256 / L rows per block at a time
+//   L = 1        whole waves, as many as the row needs (2 .. 4, a number of the launch: a wide odd row leaves less than one wave idle), blocks
+//                of 4 waves at most, so that the compiler may give a wave more than 128 registers
+//   L = 0        the same with 5 .. 16 waves, one row to a block
+// E = 8 covers 8192 elements with the 1024 lanes that a block has at most; wider rows take E = 16.
 template <typename T, int L, int E>
 struct RowShape {
     static constexpr int V = VecOf<T>::V;                       // elements per chunk
     static constexpr int K = E / V;                             // chunks per lane
-    static constexpr int THREADS = L > 64 ? L : 256;
-    static constexpr int RPB = THREADS / L;                     // rows per block and step
+    static constexpr int MAX_THREADS = L ? 256 : 1024;
+    static constexpr bool WAVES = L < 8;
+    static constexpr bool TINY = L == 8;                        // rows shorter than a chunk
+    // rows of whole waves are the same for all lanes of a wave: their addresses stay in scalar registers
+    static __device__ __forceinline__ long long row(long long r) {
+        if (!WAVES && L != 64) return r;
+        return (long long)__builtin_amdgcn_readfirstlane((int)r);      // rows < 2^31
+    }
 };
+struct RowLaunch {
+    int waves;                   // per row (L = 0)
+    int rpb;                     // rows per block and step
+    int threads;
+};
+inline RowLaunch row_launch(int L, int E, int width) {
+    if (L >= 8) return RowLaunch{1, 256 / L, 256};
+    const int w = (width + 64 * E - 1) / (64 * E), r = w < 4 ? 4 / w : 1;
+    return RowLaunch{w, r, 64 * w * r};
+}
 
-// Sums of up to N values at once over the lanes of a row, in every one of them.  `red` (2 * N * W floats) has room for two rounds: a wave
-// can be one round ahead of another, never two, so one barrier a round is enough.
-template <int L, int N>
-struct RowSum {
-    static constexpr int W = L > 64 ? L / 64 : 1;
-    float* red;
-    int turn;
-    __device__ __forceinline__ RowSum(float* r) : red(r), turn(0) {}
-    template <int M>
-    __device__ __forceinline__ void operator()(float (&v)[M]) {
-        static_assert(M <= N, "the buffer holds N values");
-#pragma unroll
-        for (int i = 0; i < M; ++i) v[i] = lane_sum<(L > 64 ? 64 : L)>(v[i]);
-        if (L > 64) {
-            float* b = red + turn * (N * W);
-            turn ^= 1;
-            if ((threadIdx.x & 63) == 0) {
-#pragma unroll
-                for (int i = 0; i < M; ++i) b[i * W + (threadIdx.x >> 6)] = v[i];
-            }
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < M; ++i) {
-                float s = 0.f;
-#pragma unroll
-                for (int k = 0; k < W; ++k) s += b[i * W + k];
-                v[i] = s;
-            }
+// This thread's place: `lane` of row group `group`
+template <int L>
+struct RowPlace {
+    int lane, group, lanes, waves;
+    __device__ __forceinline__ RowPlace(const RowLaunch& r) {
+        if (L >= 8) {
+            lane = threadIdx.x % (L >= 8 ? L : 8);
+            group = threadIdx.x / (L >= 8 ? L : 8);
+            if (L == 64) group = __builtin_amdgcn_readfirstlane(group);
+            lanes = L;
+            waves = 1;
+        } else {
+            waves = r.waves;
+            lanes = 64 * waves;
+            group = __builtin_amdgcn_readfirstlane((int)threadIdx.x / lanes);
+            lane = (int)threadIdx.x - group * lanes;
         }
     }
 };
 
-// one chunk of a parameter (or gate) that is fp32 or of the operands' type
-template <typename T>
-__device__ __forceinline__ void load_param(uint64_t p, long long at, bool f32, int n, float* v) {
-    constexpr int V = VecOf<T>::V;
-    if (f32 && V == 8) {
-        const float* q = gptr<const float>(p) + at;
-        load_chunk<float>(q, n < 4 ? n : 4, v);
-        if (n > 4) load_chunk<float>(q + 4, n - 4, v + 4);
-        else v[4] = v[5] = v[6] = v[7] = 0.f;
-    } else {
-        load_chunk<T>(gptr<const T>(p) + at, n, v);
+// Sums of up to N values at once over the lanes of a row, in every one of them.  With several waves to a row: each leaves its sums in the
+// LDS and after one barrier every wave adds them up, 16 lanes reading 16 places.  `red` (SIZE floats) has room for two rounds: a
+// wave can be one round ahead of another, never two, so one barrier a round is enough.  All threads of the block call it together.
+template <int L, int N>
+struct RowSum {
+    static constexpr int PITCH = L == 1 ? 4 * 4 : 16;           // places per value: waves of a row times rows of a block
+    static constexpr int SIZE = L < 8 ? 2 * N * PITCH : 1;
+    float* red;
+    int turn;
+    __device__ __forceinline__ RowSum(float* r) : red(r), turn(0) {}
+    template <int M>
+    __device__ __forceinline__ void operator()(float (&v)[M], const RowPlace<L>& at) {
+        static_assert(M <= N, "the buffer holds N values");
+#pragma unroll
+        for (int i = 0; i < M; ++i) v[i] = lane_sum<(L < 8 ? 64 : L)>(v[i]);
+        if (L < 8) {
+            float* b = red + turn * (N * PITCH) + at.group * at.waves;
+            turn ^= 1;
+            if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+                for (int i = 0; i < M; ++i) b[i * PITCH + (at.lane >> 6)] = v[i];
+            }
+            __syncthreads();
+            const int k = threadIdx.x & 15;
+#pragma unroll
+            for (int i = 0; i < M; ++i) v[i] = lane_sum<16>(k < at.waves ? b[i * PITCH + k] : 0.f);
+        }
     }
+};
+
+// one chunk of a row, n elements of it; TINY: the row may be shorter than a chunk
+template <typename T, bool TINY>
+__device__ __forceinline__ u32x4 load_row(const T* p, int n) {
+    return TINY ? load_raw<T>(p, n) : load_row_raw<T>(p, n);
+}
+// one chunk of a parameter (or gate) that is fp32 or of the operands' type
+template <typename T, bool TINY>
+__device__ __forceinline__ void load_param(uint64_t p, long long at, bool f32, int n, float* v) {
+    if (f32 && VecOf<T>::V == 8) {
+        const float* q = gptr<const float>(p) + at;
+        const u32x4 lo = load_row<float, TINY>(q, min(n, 4));
+        const u32x4 hi = n > 4 ? load_row<float, TINY>(q + 4, n - 4) : (u32x4){0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i] = __uint_as_float(lo[i]);
+            v[VecOf<T>::V - 4 + i] = __uint_as_float(hi[i]);
+        }
+    } else {
+        unpack16<T>(load_row<T, TINY>(gptr<const T>(p) + at, n), v);
+    }
+}
+// the same of a parameter that may be absent (then `absent`), and of a chunk that may lie behind the row (then zero)
+template <typename T, bool TINY>
+__device__ __forceinline__ void load_param_or(uint64_t p, long long at, bool f32, int n, float absent, float* v) {
+#pragma unroll
+    for (int i = 0; i < VecOf<T>::V; ++i) v[i] = p ? 0.f : absent;
+    if (p && n > 0) load_param<T, TINY>(p, at, f32, n, v);
 }
 template <typename T>
 __device__ __forceinline__ float load_param1(uint64_t p, long long at, bool f32) {
@@ -66,42 +119,56 @@ template <typename T>
 __device__ __forceinline__ void store_param(uint64_t p, long long at, bool f32, int n, const float* v) {
     if (f32 && VecOf<T>::V == 8) {
         float* q = gptr<float>(p) + at;
-        store_chunk<float>(q, n < 4 ? n : 4, v);
+        store_chunk<float>(q, n, v);
         if (n > 4) store_chunk<float>(q + 4, n - 4, v + 4);
     } else {
         store_chunk<T>(gptr<T>(p) + at, n, v);
     }
 }
 
-// act(g) and its derivative.  Both derivatives are written with e = exp(-|g|) (or its square), which keeps them exact where act(g) is
-// within a rounding of 1.
+// act(g) and its derivative of a chunk; the choice is uniform, so it stands outside the loops.  Both derivatives are written with
+// e = exp(-|g|) (or its square), which keeps them exact where act(g) is within a rounding of 1.
 __device__ __forceinline__ float gate_value(float g, int act) {
     if (act == FNET_GATE_SIGMOID) return 1.f / (1.f + __expf(-g));
     if (act == FNET_GATE_TANH) return tanhf(g);
     return g;
 }
 __device__ __forceinline__ float gate_slope(float g, int act) {
+    if (act == FNET_GATE_IDENTITY) return 1.f;
+    const float e = __expf(act == FNET_GATE_SIGMOID ? -fabsf(g) : -2.f * fabsf(g)), d = 1.f + e;
+    return (act == FNET_GATE_SIGMOID ? e : 4.f * e) / (d * d);
+}
+template <int V>
+__device__ __forceinline__ void gate_values(float* g, int act) {
     if (act == FNET_GATE_SIGMOID) {
-        const float e = __expf(-fabsf(g)), d = 1.f + e;
-        return e / (d * d);
+#pragma unroll
+        for (int i = 0; i < V; ++i) g[i] = gate_value(g[i], FNET_GATE_SIGMOID);
+    } else if (act == FNET_GATE_TANH) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) g[i] = gate_value(g[i], FNET_GATE_TANH);
     }
-    if (act == FNET_GATE_TANH) {
-        const float e = __expf(-2.f * fabsf(g)), d = 1.f + e;
-        return 4.f * e / (d * d);
+}
+template <int V>
+__device__ __forceinline__ void gate_slopes(float* g, int act) {
+    if (act == FNET_GATE_SIGMOID) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) g[i] = gate_slope(g[i], FNET_GATE_SIGMOID);
+    } else if (act == FNET_GATE_TANH) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) g[i] = gate_slope(g[i], FNET_GATE_TANH);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) g[i] = 1.f;
     }
-    return 1.f;
 }
 
 int fnet_block_norm_check(const FnetBlockNorm* a);        // the checks that both directions share
 
-// L and E by the width: E = 8 elements per lane as long as a block of at most 1024 lanes covers the row, then 16.
-#define DISPATCH_ROW(width, ...)                                                           \
-    if ((width) <= 64) { constexpr int L = 8, E = 8; __VA_ARGS__; }                         \
-    else if ((width) <= 128) { constexpr int L = 16, E = 8; __VA_ARGS__; }                  \
-    else if ((width) <= 256) { constexpr int L = 32, E = 8; __VA_ARGS__; }                  \
-    else if ((width) <= 512) { constexpr int L = 64, E = 8; __VA_ARGS__; }                  \
-    else if ((width) <= 1024) { constexpr int L = 128, E = 8; __VA_ARGS__; }                \
-    else if ((width) <= 2048) { constexpr int L = 256, E = 8; __VA_ARGS__; }                \
-    else if ((width) <= 4096) { constexpr int L = 512, E = 8; __VA_ARGS__; }                \
-    else if ((width) <= 8192) { constexpr int L = 1024, E = 8; __VA_ARGS__; }               \
-    else { constexpr int L = 1024, E = 16; __VA_ARGS__; }
+#define DISPATCH_ROW(width, ...)                                                   \
+    if ((width) <= 64) { constexpr int L = 8, E = 8; __VA_ARGS__; }                 \
+    else if ((width) <= 128) { constexpr int L = 16, E = 8; __VA_ARGS__; }          \
+    else if ((width) <= 256) { constexpr int L = 32, E = 8; __VA_ARGS__; }          \
+    else if ((width) <= 512) { constexpr int L = 64, E = 8; __VA_ARGS__; }          \
+    else if ((width) <= 2048) { constexpr int L = 1, E = 8; __VA_ARGS__; }         \
+    else if ((width) <= 8192) { constexpr int L = 0, E = 8; __VA_ARGS__; }          \
+    else { constexpr int L = 0, E = 16; __VA_ARGS__; }

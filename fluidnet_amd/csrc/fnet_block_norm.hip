@@ -3,142 +3,184 @@
 
 namespace {
 
+// How the gate enters: constant over the rows (none, per channel: part of the weight in registers), one value per row, or a row of values
+enum { GM_CONST = 0, GM_ROW = 1, GM_VECTOR = 2 };
+
 // One row: load, (mean,) sum of squares about it, the residual sum, and the same for the norm of y, all from registers; y enters the second
 // norm before it is rounded.  The variance is the mean square about the mean, not E[v^2] - mean^2, which loses everything for rows far from
-// zero.  Rows are dealt to blocks in turn; weights and scale are loaded once per block.
-template <typename T, int L, int E>
-__global__ __launch_bounds__((RowShape<T, L, E>::THREADS)) void k_block_norm_fwd(FnetBlockNorm a) {
+// zero.  Rows are dealt to blocks in turn; what multiplies a normalised value is loaded once per block.
+template <typename T, int L, int E, int GM, bool LAYER>
+__global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS)) void k_block_norm_fwd(FnetBlockNorm a, RowLaunch rl) {
     using S = RowShape<T, L, E>;
     constexpr int V = S::V, K = S::K;
-    __shared__ float red[2 * RowSum<L, 1>::W];
+    __shared__ float red[RowSum<L, 1>::SIZE];
     RowSum<L, 1> sum(red);
-    const int C = a.width, lane = threadIdx.x % L;
-    const bool pf = a.param_dtype == FNET_F32, gf = a.gate_dtype == FNET_F32, layer = a.kind == FNET_NORM_LAYER;
+    const RowPlace<L> at(rl);
+    const int C = a.width;
+    const bool pf = a.param_dtype == FNET_F32, gf = a.gate_dtype == FNET_F32;
     const float inv_c = 1.f / (float)C;
     const bool have_branch = a.branch != 0, post = a.post != 0, pre = a.h != 0;
 
-    int left[K];                                     // elements of each of this lane's chunks
-    float wpost[K][V], wpre[K][V], sc[K][V];
+    int col[K], left[K];                             // first element of each of this lane's chunks, and how many of its elements there are
+    bool full = true;
+    float wo[K][V], wy[K][V];                        // residual_scale * scale * post_weight (* act(gate)), pre_weight
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const int c = (k * L + lane) * V;
-        left[k] = min(max(C - c, 0), V);
+        col[k] = (k * at.lanes + at.lane) * V;
+        left[k] = min(max(C - col[k], 0), V);
+        full = full && left[k] == V;
+        float s[V];
+        load_param_or<T, S::TINY>(a.post_weight, col[k], pf, left[k], 1.f, wo[k]);
+        load_param_or<T, S::TINY>(a.pre_weight, col[k], pf, left[k], 1.f, wy[k]);
+        load_param_or<T, S::TINY>(a.scale, col[k], pf, left[k], 1.f, s);
 #pragma unroll
-        for (int i = 0; i < V; ++i) { wpost[k][i] = 1.f; wpre[k][i] = 1.f; sc[k][i] = a.residual_scale; }
-        if (left[k] > 0) {
-            if (a.post_weight) load_param<T>(a.post_weight, c, pf, left[k], wpost[k]);
-            if (a.pre_weight) load_param<T>(a.pre_weight, c, pf, left[k], wpre[k]);
-            if (a.scale) {
-                load_param<T>(a.scale, c, pf, left[k], sc[k]);
+        for (int i = 0; i < V; ++i) wo[k][i] *= a.residual_scale * s[i];
+        if (GM == GM_CONST && a.gate) {
+            load_param_or<T, S::TINY>(a.gate, col[k], gf, left[k], 1.f, s);
+            gate_values<V>(s, a.gate_act);
 #pragma unroll
-                for (int i = 0; i < V; ++i) sc[k][i] *= a.residual_scale;
-            }
+            for (int i = 0; i < V; ++i) wo[k][i] *= s[i];
         }
     }
+    full = __all(full);                              // of this wave: no element of its chunks lies behind the row
 
-    for (long long row = (long long)blockIdx.x * S::RPB + threadIdx.x / L; row < a.rows; row += (long long)gridDim.x * S::RPB) {
-        float y[K][V], o[K][V];
-        const T* px = gptr<const T>(a.x) + row * a.x_stride;
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int c = (k * L + lane) * V;
-#pragma unroll
-            for (int i = 0; i < V; ++i) { y[k][i] = 0.f; o[k][i] = 0.f; }
-            if (left[k] > 0) {
-                load_chunk<T>(px + c, left[k], y[k]);
-                if (have_branch) load_chunk<T>(gptr<const T>(a.branch) + row * a.branch_stride + c, left[k], o[k]);
-            }
-        }
-        float v1[1];
-        auto statistics = [&](float (&v)[K][V], float& mu, float& r) {
-            mu = 0.f;
-            if (layer) {
-                v1[0] = 0.f;
-#pragma unroll
-                for (int k = 0; k < K; ++k)
-#pragma unroll
-                    for (int i = 0; i < V; ++i) v1[0] += i < left[k] ? v[k][i] : 0.f;   // behind the row lies the norm of zeros
-                sum(v1);
-                mu = v1[0] * inv_c;
-            }
-            v1[0] = 0.f;
+    // 1 / deviation of a row (and its mean, taken off)
+    auto normalise = [&](float (&v)[K][V], float& mu) {
+        float s[1];
+        mu = 0.f;
+        if (LAYER) {
+            s[0] = 0.f;
 #pragma unroll
             for (int k = 0; k < K; ++k)
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float d = i < left[k] ? v[k][i] - mu : 0.f;
-                    v1[0] = fmaf(d, d, v1[0]);
-                }
-            sum(v1);
-            r = 1.f / sqrtf(v1[0] * inv_c + a.eps);
-        };
-        if (have_branch) {
-            if (post) {
-                float mu, r;
-                statistics(o, mu, r);
-                if (a.stats && lane == 0) {
-                    gptr<float>(a.stats)[row] = mu;
-                    gptr<float>(a.stats)[a.rows + row] = r;
-                }
+                for (int i = 0; i < V; ++i) s[0] += v[k][i];
+            sum(s, at);
+            mu = s[0] * inv_c;
 #pragma unroll
-                for (int k = 0; k < K; ++k) {
+            for (int k = 0; k < K; ++k)
 #pragma unroll
-                    for (int i = 0; i < V; ++i) o[k][i] = (o[k][i] - mu) * r * wpost[k][i];
-                    if (a.post_bias && left[k] > 0) {
-                        float b[V];
-                        load_param<T>(a.post_bias, (k * L + lane) * V, pf, left[k], b);
-#pragma unroll
-                        for (int i = 0; i < V; ++i) o[k][i] += b[i];
-                    }
-                }
-            }
-            if (a.gate_kind == FNET_GATE_TOKEN) {
-                const float g = gate_value(load_param1<T>(a.gate, row * a.gate_stride, gf), a.gate_act);
+                for (int i = 0; i < V; ++i) v[k][i] -= mu;
+            if (!full) {
 #pragma unroll
                 for (int k = 0; k < K; ++k)
 #pragma unroll
-                    for (int i = 0; i < V; ++i) o[k][i] *= g;
-            } else if (a.gate_kind != FNET_GATE_NONE) {
-                const long long at = a.gate_kind == FNET_GATE_ELEMENT ? row * a.gate_stride
-                                     : a.gate_kind == FNET_GATE_SAMPLE ? (long long)((uint32_t)row / (uint32_t)a.tokens) * a.gate_stride : 0;
-#pragma unroll
-                for (int k = 0; k < K; ++k) {
-                    if (left[k] <= 0) continue;
-                    float g[V];
-                    load_param<T>(a.gate, at + (k * L + lane) * V, gf, left[k], g);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) o[k][i] *= gate_value(g[i], a.gate_act);
-                }
+                    for (int i = 0; i < V; ++i) v[k][i] = i < left[k] ? v[k][i] : 0.f;
             }
-            T* py = gptr<T>(a.y) + row * (long long)C;
+        }
+        s[0] = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) s[0] = fmaf(v[k][i], v[k][i], s[0]);
+        sum(s, at);
+        return 1.f / sqrtf(s[0] * inv_c + a.eps);
+    };
+
+    // several waves to a row go through the barriers of its sums together: a block's groups take the same number of steps
+    for (long long first = (long long)blockIdx.x * rl.rpb; first < a.rows; first += (long long)gridDim.x * rl.rpb) {
+        const long long row = S::row(first + at.group);
+        const bool here = row < a.rows;
+        if (!S::WAVES && !here) break;
+        float y[K][V], o[K][V];
+        {
+            u32x4 rx[K], ro[K];
 #pragma unroll
             for (int k = 0; k < K; ++k) {
+                rx[k] = ro[k] = (u32x4){0u, 0u, 0u, 0u};
+                if (here && left[k] > 0) {
+                    rx[k] = load_row<T, S::TINY>(gptr<const T>(a.x) + row * a.x_stride + col[k], left[k]);
+                    if (have_branch) ro[k] = load_row<T, S::TINY>(gptr<const T>(a.branch) + row * a.branch_stride + col[k], left[k]);
+                }
+            }
 #pragma unroll
-                for (int i = 0; i < V; ++i) y[k][i] = fmaf(sc[k][i], o[k][i], y[k][i]);
-                if (left[k] > 0) store_chunk<T>(py + (k * L + lane) * V, left[k], y[k]);
+            for (int k = 0; k < K; ++k) {
+                unpack16<T>(rx[k], y[k]);
+                unpack16<T>(ro[k], o[k]);
+            }
+        }
+        if (have_branch) {
+            float r = 1.f, mu = 0.f, gt = 1.f;
+            if (GM == GM_ROW && here) gt = gate_value(load_param1<T>(a.gate, row * a.gate_stride, gf), a.gate_act);
+            if (post) {
+                r = normalise(o, mu);
+                if (a.stats && here && at.lane == 0) {
+                    gptr<float>(a.stats)[row] = mu;
+                    gptr<float>(a.stats)[a.rows + row] = r;
+                }
+            }
+            const long long gate_at = GM != GM_VECTOR ? 0 : a.gate_kind == FNET_GATE_ELEMENT ? row * a.gate_stride
+                                      : (long long)((uint32_t)row / (uint32_t)a.tokens) * a.gate_stride;
+            const float rg = GM == GM_ROW ? r * gt : r;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                float g[V], b[V];
+                if (GM == GM_VECTOR) {
+                    load_param_or<T, S::TINY>(a.gate, gate_at + col[k], gf, here ? left[k] : 0, 0.f, g);
+                    gate_values<V>(g, a.gate_act);
+                }
+                if (a.post_bias) {                   // (v r w + b) = (v r) w + b, with the gate and scale on both
+                    float s[V];
+                    load_param_or<T, S::TINY>(a.post_bias, col[k], pf, left[k], 0.f, b);
+                    load_param_or<T, S::TINY>(a.scale, col[k], pf, left[k], 1.f, s);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) b[i] *= a.residual_scale * s[i];
+                    if (GM == GM_CONST && a.gate) {
+                        load_param_or<T, S::TINY>(a.gate, col[k], gf, left[k], 1.f, s);
+                        gate_values<V>(s, a.gate_act);
+#pragma unroll
+                        for (int i = 0; i < V; ++i) b[i] *= s[i];
+                    }
+                    if (GM == GM_ROW) {
+#pragma unroll
+                        for (int i = 0; i < V; ++i) b[i] *= gt;
+                    }
+#pragma unroll
+                    for (int i = 0; i < V; ++i) o[k][i] = fmaf(o[k][i] * rg, wo[k][i], b[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) o[k][i] = o[k][i] * rg * wo[k][i];
+                }
+#pragma unroll
+                for (int i = 0; i < V; ++i) y[k][i] = GM == GM_VECTOR ? fmaf(o[k][i], g[i], y[k][i]) : y[k][i] + o[k][i];
+                if (here && left[k] > 0) store_chunk<T>(gptr<T>(a.y) + row * (long long)C + col[k], left[k], y[k]);
             }
         }
         if (pre) {
-            float mu, r;
-            statistics(y, mu, r);
-            if (a.stats && lane == 0) {
+            float mu;
+            const float r = normalise(y, mu);
+            if (a.stats && here && at.lane == 0) {
                 gptr<float>(a.stats)[2 * a.rows + row] = mu;
                 gptr<float>(a.stats)[3 * a.rows + row] = r;
             }
-            T* ph = gptr<T>(a.h) + row * (long long)C;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                if (left[k] <= 0) continue;
-                float b[V];
+                if (a.pre_bias) {
+                    float b[V];
+                    load_param_or<T, S::TINY>(a.pre_bias, col[k], pf, left[k], 0.f, b);
 #pragma unroll
-                for (int i = 0; i < V; ++i) b[i] = 0.f;
-                if (a.pre_bias) load_param<T>(a.pre_bias, (k * L + lane) * V, pf, left[k], b);
+                    for (int i = 0; i < V; ++i) y[k][i] = fmaf(y[k][i] * r, wy[k][i], b[i]);
+                } else {
 #pragma unroll
-                for (int i = 0; i < V; ++i) b[i] = fmaf((y[k][i] - mu) * r, wpre[k][i], b[i]);
-                store_chunk<T>(ph + (k * L + lane) * V, left[k], b);
+                    for (int i = 0; i < V; ++i) y[k][i] = y[k][i] * r * wy[k][i];
+                }
+                if (here && left[k] > 0) store_chunk<T>(gptr<T>(a.h) + row * (long long)C + col[k], left[k], y[k]);
             }
         }
     }
+}
+
+template <typename T, int L, int E>
+void run_fwd(const FnetBlockNorm& a, int gm, hipStream_t st) {
+    const RowLaunch rl = row_launch(L, E, a.width);
+    const long long steps = (a.rows + rl.rpb - 1) / rl.rpb;
+    const long long most = 256 * (2048 / rl.threads);                  // what the chip holds at once
+    const dim3 grid((unsigned)(steps < most ? steps : most)), block(rl.threads);
+    const bool layer = a.kind == FNET_NORM_LAYER;
+#define FNET_FWD(GM, LAYER) hipLaunchKernelGGL((k_block_norm_fwd<T, L, E, GM, LAYER>), grid, block, 0, st, a, rl)
+    if (gm == GM_CONST) { if (layer) FNET_FWD(GM_CONST, true); else FNET_FWD(GM_CONST, false); }
+    else if (gm == GM_ROW) { if (layer) FNET_FWD(GM_ROW, true); else FNET_FWD(GM_ROW, false); }
+    else { if (layer) FNET_FWD(GM_VECTOR, true); else FNET_FWD(GM_VECTOR, false); }
+#undef FNET_FWD
 }
 
 bool type_ok(int d, int operand) { return d == FNET_F32 || d == operand; }
@@ -172,12 +214,8 @@ int fnet_block_norm_fwd(const FnetBlockNorm* host_args, void* stream) {
     if (a.rows == 0) return FNET_OK;
     FNET_CHECK_ARG((a.branch != 0) == (a.y != 0) && (a.y != 0 || a.h != 0) && (a.h != 0 || (a.pre_weight == 0 && a.pre_bias == 0)));
     FNET_CHECK_ARG(aligned(a.y | a.h, a.dtype));
-    DISPATCH_T3(a.dtype, DISPATCH_ROW(a.width, {
-        using S = RowShape<T, L, E>;
-        const long long steps = (a.rows + S::RPB - 1) / S::RPB;
-        const long long most = 256 * (2048 / S::THREADS);              // what the chip holds at once
-        hipLaunchKernelGGL((k_block_norm_fwd<T, L, E>), dim3((unsigned)(steps < most ? steps : most)), dim3(S::THREADS), 0, (hipStream_t)stream, a);
-    }));
+    const int gm = a.gate_kind == FNET_GATE_TOKEN ? GM_ROW : a.gate_kind == FNET_GATE_ELEMENT || a.gate_kind == FNET_GATE_SAMPLE ? GM_VECTOR : GM_CONST;
+    DISPATCH_T3(a.dtype, DISPATCH_ROW(a.width, { run_fwd<T, L, E>(a, gm, (hipStream_t)stream); }));
     FNET_LAUNCH_CHECK();
     return FNET_OK;
 }

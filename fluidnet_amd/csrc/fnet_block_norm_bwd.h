@@ -1,0 +1,351 @@
+// The backward kernel of the norms around a residual block, for one operand type; fnet_block_norm_bwd_{f32,bf16,f16}.hip instantiate it.
+#pragma once
+#include "fnet_block_norm.h"
+
+// gradients that are sums over rows
+enum { SUM_PRE_W = 0, SUM_PRE_B, SUM_POST_W, SUM_POST_B, SUM_SCALE, SUM_GATE, SUM_COUNT };
+
+struct BwdPlan {
+    uint64_t dst[SUM_COUNT];     // where a block leaves a sum: its row of the partial sums, or (direct) the gradient itself; 0: nowhere
+    int direct;                  // bit i: dst[i] is the gradient, in its own type
+    // the sums of the branch's side are left per segment (a sample's gate is part of them), those of the second norm per block; only with a
+    // gate per sample does a block go through several segments
+    int samples, parts;          // segments = samples * parts: part p of a sample is its rows [p * part_rows, (p + 1) * part_rows)
+    long long sample_rows, part_rows;
+};
+
+// How the gate enters: constant over a segment's rows (none, per channel, per sample), one value per row, or a row of values per row
+enum { GM_CONST = 0, GM_ROW = 1, GM_VECTOR = 2 };
+
+// Waves per SIMD that the kernel is compiled for: 4 leave 128 registers to each; two more sums or a gate in registers do not fit those, and
+// 3 waves without spilling are faster than 4 with it.  Blocks of more than 8 waves leave no choice.
+constexpr int bwd_waves(int L, int gm, bool bias) { return (bias || gm == GM_VECTOR) && L != 0 ? 3 : 4; }
+
+// one instance: launches the kernel (bias: sums for biases too)
+template <typename T, int L, int E>
+void fnet_block_norm_bwd_launch(const FnetBlockNorm& a, const BwdPlan& plan, const RowLaunch& rl, int blocks, int gm, bool bias, hipStream_t st);
+
+#ifdef FNET_BLOCK_NORM_BWD_KERNEL
+namespace {
+
+// The sums of a block's row groups into row `row` of `dst`: through LDS, group by group in order.
+template <typename T, int L, int E>
+__device__ __forceinline__ void leave_sum(const float (&acc)[RowShape<T, L, E>::K][RowShape<T, L, E>::V], uint64_t dst, long long row, int C,
+                                          bool direct, bool f32, float* sm, const RowPlace<L>& at, int groups) {
+    constexpr int V = RowShape<T, L, E>::V, K = RowShape<T, L, E>::K;
+    if (groups == 1) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int c = (k * at.lanes + at.lane) * V, n = min(C - c, V);
+            if (n <= 0) continue;
+            if (direct) {
+                store_param<T>(dst, row * C + c, f32, n, acc[k]);
+            } else {
+                float* q = gptr<float>(dst) + row * C + c;
+#pragma unroll
+                for (int i = 0; i < V; i += 4)
+                    if (n > i) store_chunk<float>(q + i, n - i, &acc[k][i]);
+            }
+        }
+        return;
+    }
+    const int pitch = at.lanes * E;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) sm[at.group * pitch + (k * at.lanes + at.lane) * V + i] = acc[k][i];
+    __syncthreads();
+    for (int c = threadIdx.x; c < C; c += blockDim.x) {
+        float s = 0.f;
+        for (int g = 0; g < groups; ++g) s += sm[g * pitch + c];
+        if (direct && !f32) gptr<T>(dst)[row * C + c] = f_to_elem<T>(s);
+        else gptr<float>(dst)[row * C + c] = s;
+    }
+}
+
+// With z the normalised branch (or the branch itself), W = residual_scale * scale * post_weight, B = residual_scale * scale * post_bias and
+// f = act(gate):   y = x + f (W z + B),   d = gradient of y (of the row's own dy and of h through the second norm)
+//   dbranch: q = f d W through the norm;    dgate = act'(gate) d (W z + B)
+//   dpost_weight = residual_scale * scale * sum f d z,  dpost_bias = residual_scale * scale * sum f d,
+//   dscale = residual_scale * (post_weight * sum f d z + post_bias * sum f d)
+// so two sums over rows (one without biases) give every gradient on the branch's side, and where f is constant over the rows it enters only
+// when they are left: f is part of W and B in registers, and dgate of a channel or sample comes from the same two sums.
+// A row's arithmetic is 18 to 40 operations an element, which keeps it below the time of the 10 to 14 bytes it moves (bf16).
+template <typename T, int L, int E, int GM, bool LAYER, bool BIAS>
+__global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, BIAS)) void k_block_norm_bwd(FnetBlockNorm a, BwdPlan plan, RowLaunch rl) {
+    using S = RowShape<T, L, E>;
+    constexpr int V = S::V, K = S::K;
+    __shared__ float red[RowSum<L, 3>::SIZE];
+    __shared__ float sm[L ? 256 * E : 1];            // several row groups: 256 lanes
+    RowSum<L, 3> sum(red);
+    const RowPlace<L> at(rl);
+    const int C = a.width, groups = rl.rpb;
+    const bool pf = a.param_dtype == FNET_F32, gf = a.gate_dtype == FNET_F32;
+    const float inv_c = 1.f / (float)C;
+    const bool post = a.post != 0, pre = a.dh != 0;
+    // the branch is read for y (through the second norm) and for the gradients on its side
+    const bool branch_grads = a.branch != 0 && (a.dbranch || a.dgate || a.dscale || a.dpost_weight || a.dpost_bias);
+    const bool need_branch = a.branch != 0 && (pre || branch_grads);
+
+    int col[K], left[K];
+    bool full = true;
+    float wy[K][V], wo[K][V], bo[BIAS ? K : 1][V];    // pre_weight; W and B above (with f, where that is constant)
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        col[k] = (k * at.lanes + at.lane) * V;
+        left[k] = min(max(C - col[k], 0), V);
+        full = full && left[k] == V;
+        load_param_or<T, S::TINY>(a.pre_weight, col[k], pf, left[k], 1.f, wy[k]);
+    }
+    full = __all(full);
+    auto load_branch_side = [&](long long gate_at) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float s[V];
+            load_param_or<T, S::TINY>(a.scale, col[k], pf, left[k], 1.f, s);
+#pragma unroll
+            for (int i = 0; i < V; ++i) s[i] *= a.residual_scale;
+            if (GM == GM_CONST && a.gate) {
+                float g[V];
+                load_param_or<T, S::TINY>(a.gate, gate_at + col[k], gf, left[k], 1.f, g);
+                gate_values<V>(g, a.gate_act);
+#pragma unroll
+                for (int i = 0; i < V; ++i) s[i] *= g[i];
+            }
+            load_param_or<T, S::TINY>(a.post_weight, col[k], pf, left[k], 1.f, wo[k]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) wo[k][i] *= s[i];
+            if (BIAS) {
+                load_param_or<T, S::TINY>(a.post_bias, col[k], pf, left[k], 0.f, bo[BIAS ? k : 0]);
+#pragma unroll
+                for (int i = 0; i < V; ++i) bo[BIAS ? k : 0][i] *= s[i];
+            }
+        }
+    };
+
+    float ay[K][V], ay0[BIAS ? K : 1][V], ao[K][V], ao0[BIAS ? K : 1][V];       // sums of dh y_hat, dh, f d z, f d
+    auto clear = [](auto& s) {
+        for (auto& r : s)
+            for (auto& e : r) e = 0.f;
+    };
+    clear(ay);
+    clear(ay0);
+    clear(ao);
+    clear(ao0);
+
+    // the branch's sums, each times its factor (see above), to row `to` of their destinations
+    auto leave_branch_sums = [&](long long to, long long gate_at) {
+#pragma unroll 1
+        for (int s = SUM_POST_W; s < SUM_COUNT; ++s) {
+            if (!plan.dst[s]) continue;
+            float v[K][V];
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                float sc[V], w[V], b[V], g[V];
+                load_param_or<T, S::TINY>(a.scale, col[k], pf, left[k], 1.f, sc);
+                load_param_or<T, S::TINY>(a.post_weight, col[k], pf, left[k], 1.f, w);
+                load_param_or<T, S::TINY>(a.post_bias, col[k], pf, left[k], 0.f, b);
+                load_param_or<T, S::TINY>(GM == GM_CONST ? a.gate : 0, gate_at + col[k], gf, left[k], 1.f, g);
+                if (GM == GM_CONST && a.gate) {
+                    if (s == SUM_GATE) gate_slopes<V>(g, a.gate_act);
+                    else gate_values<V>(g, a.gate_act);
+                }
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float p0 = BIAS ? ao0[BIAS ? k : 0][i] : 0.f;
+                    const float m = s == SUM_POST_W ? ao[k][i] : s == SUM_POST_B ? p0 : w[i] * ao[k][i] + b[i] * p0;
+                    v[k][i] = a.residual_scale * (s == SUM_SCALE ? 1.f : sc[i]) * g[i] * m;
+                }
+            }
+            leave_sum<T, L, E>(v, plan.dst[s], to, C, (plan.direct >> s) & 1, s == SUM_GATE ? gf : pf, sm, at, groups);
+        }
+    };
+
+    const int segments = plan.samples * plan.parts;
+    for (int seg = blockIdx.x; seg < segments; seg += gridDim.x) {
+        const int sample = seg / plan.parts;
+        const long long first = sample * plan.sample_rows + (seg - sample * plan.parts) * plan.part_rows;
+        const long long end = min(first + plan.part_rows, (sample + 1) * plan.sample_rows);
+        const long long sample_gate = a.gate_kind == FNET_GATE_SAMPLE ? (long long)sample * a.gate_stride : 0;
+        load_branch_side(sample_gate);
+        // several waves to a row go through the barriers of its sums together: a block's groups take the same number of steps
+        for (long long step = first; step < end; step += groups) {
+            const long long row = S::row(step + at.group);
+            const bool here = row < end;
+            if (!S::WAVES && !here) break;
+            u32x4 rx[K], ro[K], rd[K], rt[K];
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                rx[k] = ro[k] = rd[k] = rt[k] = (u32x4){0u, 0u, 0u, 0u};
+                if (here && left[k] > 0) {
+                    if (pre) {
+                        rt[k] = load_row<T, S::TINY>(gptr<const T>(a.dh) + row * a.dh_stride + col[k], left[k]);
+                        rx[k] = load_row<T, S::TINY>(gptr<const T>(a.x) + row * a.x_stride + col[k], left[k]);
+                    }
+                    if (need_branch) ro[k] = load_row<T, S::TINY>(gptr<const T>(a.branch) + row * a.branch_stride + col[k], left[k]);
+                    if (a.dy) rd[k] = load_row<T, S::TINY>(gptr<const T>(a.dy) + row * a.dy_stride + col[k], left[k]);
+                }
+            }
+            float mu_o = 0.f, r_o = 1.f, mu_y = 0.f, r_y = 1.f, gt = 0.f, ft = 1.f;
+            if (here) {
+                if (post) { mu_o = gptr<const float>(a.stats)[row]; r_o = gptr<const float>(a.stats)[a.rows + row]; }
+                if (pre) { mu_y = gptr<const float>(a.stats)[2 * a.rows + row]; r_y = gptr<const float>(a.stats)[3 * a.rows + row]; }
+                if (GM == GM_ROW) {
+                    gt = load_param1<T>(a.gate, row * a.gate_stride, gf);
+                    ft = gate_value(gt, a.gate_act);
+                }
+            }
+            float z[K][V], d[K][V], f[GM == GM_VECTOR ? K : 1][V];
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                unpack16<T>(ro[k], z[k]);
+                if (GM == GM_VECTOR) {
+                    float(&fk)[V] = f[GM == GM_VECTOR ? k : 0];
+                    load_param_or<T, S::TINY>(a.gate, row * a.gate_stride + col[k], gf, here ? left[k] : 0, 0.f, fk);
+                    gate_values<V>(fk, a.gate_act);
+                }
+                if (post) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) z[k][i] = LAYER ? (z[k][i] - mu_o) * r_o : z[k][i] * r_o;
+                }
+            }
+            if (!pre) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) unpack16<T>(rd[k], d[k]);
+            } else {
+                float y[K][V], t[K][V], s2[2] = {0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    unpack16<T>(rx[k], y[k]);
+                    unpack16<T>(rt[k], t[k]);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        if (GM == GM_CONST) {
+                            y[k][i] = fmaf(wo[k][i], z[k][i], BIAS ? y[k][i] + bo[BIAS ? k : 0][i] : y[k][i]);
+                        } else {
+                            const float u = BIAS ? fmaf(wo[k][i], z[k][i], bo[BIAS ? k : 0][i]) : wo[k][i] * z[k][i];
+                            y[k][i] = fmaf(GM == GM_ROW ? ft : f[GM == GM_VECTOR ? k : 0][i], u, y[k][i]);
+                        }
+                        y[k][i] = LAYER ? (y[k][i] - mu_y) * r_y : y[k][i] * r_y;
+                        ay[k][i] = fmaf(t[k][i], y[k][i], ay[k][i]);
+                        if (BIAS) ay0[BIAS ? k : 0][i] += t[k][i];
+                        t[k][i] *= wy[k][i];
+                        if (LAYER) s2[0] += t[k][i];
+                        s2[1] = fmaf(t[k][i], y[k][i], s2[1]);
+                    }
+                }
+                if (LAYER) {
+                    sum(s2, at);
+                } else {
+                    float s1[1] = {s2[1]};
+                    sum(s1, at);
+                    s2[1] = s1[0];
+                }
+                const float m0 = LAYER ? s2[0] * inv_c : 0.f, m1 = s2[1] * inv_c;
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    unpack16<T>(rd[k], d[k]);        // held as loaded until here: registers are what limits the waves in flight
+#pragma unroll
+                    for (int i = 0; i < V; ++i) d[k][i] = fmaf(r_y, fmaf(-m1, y[k][i], LAYER ? t[k][i] - m0 : t[k][i]), d[k][i]);
+                }
+            }
+            if (!full) {
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) d[k][i] = i < left[k] ? d[k][i] : 0.f;
+            }
+            if (a.dx) {
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+                    if (here && left[k] > 0) store_chunk<T>(gptr<T>(a.dx) + row * (long long)C + col[k], left[k], d[k]);
+            }
+            if (branch_grads) {
+                float s3[3] = {0.f, 0.f, 0.f};       // sums of q, q z and, per row, d B; q = d W, with the row's f put in after the sums
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    if (GM == GM_VECTOR) {
+                        float(&fk)[V] = f[GM == GM_VECTOR ? k : 0];
+                        if (a.dgate) {
+                            float g[V];
+                            load_param_or<T, S::TINY>(a.gate, row * a.gate_stride + col[k], gf, here ? left[k] : 0, 0.f, g);
+                            gate_slopes<V>(g, a.gate_act);
+#pragma unroll
+                            for (int i = 0; i < V; ++i) g[i] *= d[k][i] * (BIAS ? fmaf(wo[k][i], z[k][i], bo[BIAS ? k : 0][i]) : wo[k][i] * z[k][i]);
+                            if (here && left[k] > 0) store_param<T>(a.dgate, row * (long long)C + col[k], gf, left[k], g);
+                        }
+#pragma unroll
+                        for (int i = 0; i < V; ++i) d[k][i] *= fk[i];
+                    }
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float fd = GM == GM_ROW ? ft * d[k][i] : d[k][i];
+                        ao[k][i] = fmaf(fd, z[k][i], ao[k][i]);
+                        if (BIAS) ao0[BIAS ? k : 0][i] += fd;
+                        if (GM == GM_ROW && BIAS) s3[2] = fmaf(d[k][i], bo[BIAS ? k : 0][i], s3[2]);
+                        d[k][i] *= wo[k][i];
+                        if (LAYER) s3[0] += d[k][i];
+                        s3[1] = fmaf(d[k][i], z[k][i], s3[1]);
+                    }
+                }
+                if (post || GM == GM_ROW) sum(s3, at);
+                if (GM == GM_ROW && a.dgate && here && at.lane == 0) {
+                    const float dg = gate_slope(gt, a.gate_act) * (s3[1] + s3[2]);
+                    if (gf) gptr<float>(a.dgate)[row] = dg;
+                    else gptr<T>(a.dgate)[row] = f_to_elem<T>(dg);
+                }
+                if (a.dbranch) {
+                    const float m0 = LAYER ? s3[0] * inv_c : 0.f, m1 = s3[1] * inv_c, r = r_o * ft;
+#pragma unroll
+                    for (int k = 0; k < K; ++k) {
+                        if (post) {
+#pragma unroll
+                            for (int i = 0; i < V; ++i) d[k][i] = r * fmaf(-m1, z[k][i], LAYER ? d[k][i] - m0 : d[k][i]);
+                        } else if (GM == GM_ROW) {
+#pragma unroll
+                            for (int i = 0; i < V; ++i) d[k][i] *= ft;
+                        }
+                        if (here && left[k] > 0) store_chunk<T>(gptr<T>(a.dbranch) + row * (long long)C + col[k], left[k], d[k]);
+                    }
+                }
+            }
+        }
+        leave_branch_sums(seg, sample_gate);
+        clear(ao);
+        clear(ao0);
+    }
+    if (plan.dst[SUM_PRE_W]) leave_sum<T, L, E>(ay, plan.dst[SUM_PRE_W], blockIdx.x, C, (plan.direct >> SUM_PRE_W) & 1, pf, sm, at, groups);
+    if (BIAS && plan.dst[SUM_PRE_B]) {
+        float v[K][V];
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[k][i] = ay0[BIAS ? k : 0][i];
+        leave_sum<T, L, E>(v, plan.dst[SUM_PRE_B], blockIdx.x, C, (plan.direct >> SUM_PRE_B) & 1, pf, sm, at, groups);
+    }
+}
+
+}  // namespace
+
+template <typename T, int L, int E>
+void fnet_block_norm_bwd_launch(const FnetBlockNorm& a, const BwdPlan& plan, const RowLaunch& rl, int blocks, int gm, bool bias, hipStream_t st) {
+    const dim3 grid(blocks), block(rl.threads);
+    const bool layer = a.kind == FNET_NORM_LAYER;
+#define FNET_BWD3(GM, LAYER, BIAS) hipLaunchKernelGGL((k_block_norm_bwd<T, L, E, GM, LAYER, BIAS>), grid, block, 0, st, a, plan, rl)
+#define FNET_BWD(GM)                                                                    \
+    if (layer) { if (bias) FNET_BWD3(GM, true, true); else FNET_BWD3(GM, true, false); } \
+    else { if (bias) FNET_BWD3(GM, false, true); else FNET_BWD3(GM, false, false); }
+    if (gm == GM_CONST) { FNET_BWD(GM_CONST) }
+    else if (gm == GM_ROW) { FNET_BWD(GM_ROW) }
+    else { FNET_BWD(GM_VECTOR) }
+#undef FNET_BWD
+#undef FNET_BWD3
+}
+#define FNET_BLOCK_NORM_BWD_INSTANCE(T, L, E)                                                                                          \
+    template void fnet_block_norm_bwd_launch<T, L, E>(const FnetBlockNorm&, const BwdPlan&, const RowLaunch&, int, int, bool, hipStream_t);
+#define FNET_BLOCK_NORM_BWD_INSTANCES(T)                                                              \
+    FNET_BLOCK_NORM_BWD_INSTANCE(T, 8, 8) FNET_BLOCK_NORM_BWD_INSTANCE(T, 16, 8)                       \
+    FNET_BLOCK_NORM_BWD_INSTANCE(T, 32, 8) FNET_BLOCK_NORM_BWD_INSTANCE(T, 64, 8)                      \
+    FNET_BLOCK_NORM_BWD_INSTANCE(T, 1, 8) FNET_BLOCK_NORM_BWD_INSTANCE(T, 0, 8) FNET_BLOCK_NORM_BWD_INSTANCE(T, 0, 16)
+#endif

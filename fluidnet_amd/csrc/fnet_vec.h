@@ -72,42 +72,81 @@ template <> __device__ __forceinline__ u32x4 pack16<f16_t>(const float* v) {
 
 // n (1 .. V) leading elements of the 16-byte chunk at p; the rest reads as zero / is left alone
 template <typename T>
-__device__ __forceinline__ void load_chunk(const T* p, int n, float* v) {
+__device__ __forceinline__ u32x4 load_raw(const T* p, int n) {
     constexpr int V = VecOf<T>::V;
-    if (n >= V) {
-        const u32x4 w = *reinterpret_cast<const typename VecOf<T>::vec*>(p);
-        unpack16<T>(w, v);
-    } else {
+    if (n >= V) return *reinterpret_cast<const typename VecOf<T>::vec*>(p);
+    u32x4 w = {0u, 0u, 0u, 0u};
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[k] = k < n ? elem_to_f<T>(p[k]) : 0.f;
+    for (int k = 0; k < V; ++k) {
+        if (k >= n) break;
+        if (V == 4) w[k] = reinterpret_cast<const uint32_t*>(p)[k];
+        else w[k / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(p)[k] << (16 * (k & 1));
     }
+    return w;
 }
+template <typename T>
+__device__ __forceinline__ void load_chunk(const T* p, int n, float* v) { unpack16<T>(load_raw<T>(p, n), v); }
 template <typename T>
 __device__ __forceinline__ void store_chunk(T* p, int n, const float* v) {
     constexpr int V = VecOf<T>::V;
+    const u32x4 w = pack16<T>(v);
     if (n >= V) {
-        *reinterpret_cast<typename VecOf<T>::vec*>(p) = pack16<T>(v);
-    } else {
-#pragma unroll
-        for (int k = 0; k < V; ++k)
-            if (k < n) p[k] = f_to_elem<T>(v[k]);
+        *reinterpret_cast<typename VecOf<T>::vec*>(p) = w;
+        return;
     }
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        if (k >= n) break;
+        if (V == 4) reinterpret_cast<uint32_t*>(p)[k] = w[k];
+        else reinterpret_cast<uint16_t*>(p)[k] = (uint16_t)(w[k / 2] >> (16 * (k & 1)));
+    }
+}
+
+// The same for a chunk that ends a row of at least V elements: the 16 bytes that end where the row ends, shifted down to the chunk's own
+// place (one load and a dozen operations instead of a load per element).
+template <typename T>
+__device__ __forceinline__ u32x4 load_row_raw(const T* p, int n) {
+    constexpr int V = VecOf<T>::V;
+    const int s = V - n;                             // 0 for a whole chunk
+    u32x4 w = *reinterpret_cast<const typename VecOf<T>::vec*>(p - s);
+    if (s) {
+        if (V == 8) {
+            const u32x4 h = {__builtin_amdgcn_alignbit(w[1], w[0], 16), __builtin_amdgcn_alignbit(w[2], w[1], 16),
+                             __builtin_amdgcn_alignbit(w[3], w[2], 16), w[3] >> 16};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = (s & 1) ? h[k] : w[k];
+        }
+        const int d = V == 8 ? s >> 1 : s;           // in words
+        const u32x4 one = {w[1], w[2], w[3], 0u};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = (d & 1) ? one[k] : w[k];
+        const u32x4 two = {w[2], w[3], 0u, 0u};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = (d & 2) ? two[k] : w[k];
+    }
+    return w;
 }
 
 // Sum over groups of L consecutive lanes (L = 8 .. 64, a power of two), the result in every lane of the group.  Inside 16 lanes by DPP:
 // quad_perm exchanges neighbours and pairs, and once a group of four (eight) holds one value the half mirror (mirror) exchanges groups.
-template <int CTRL>
+// Above, row_bcast carries a 16-lane sum on and the group's last lane is read: no trip through the LDS.
+template <int CTRL, int ROWS = 0xf>
 __device__ __forceinline__ float dpp_f(float v) {
-    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true));
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, ROWS, 0xf, ROWS == 0xf));
+}
+__device__ __forceinline__ float read_lane(float v, int lane) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), lane));
 }
 template <int L>
 __device__ __forceinline__ float lane_sum(float v) {
-    v += dpp_f<0xB1>(v);                 // quad_perm [1,0,3,2]
-    v += dpp_f<0x4E>(v);                 // quad_perm [2,3,0,1]
-    if (L >= 8) v += dpp_f<0x141>(v);    // row_half_mirror
-    if (L >= 16) v += dpp_f<0x140>(v);   // row_mirror
-    if (L >= 32) v += __shfl_xor(v, 16, 64);
-    if (L >= 64) v += __shfl_xor(v, 32, 64);
+    v += dpp_f<0xB1>(v);                            // quad_perm [1,0,3,2]
+    v += dpp_f<0x4E>(v);                            // quad_perm [2,3,0,1]
+    v += dpp_f<0x141>(v);                           // row_half_mirror
+    if (L >= 16) v += dpp_f<0x140>(v);              // row_mirror
+    if (L >= 32) v += dpp_f<0x142, 0xa>(v);         // row_bcast15 into rows 1 and 3
+    if (L >= 64) v += dpp_f<0x143, 0xc>(v);         // row_bcast31 into rows 2 and 3
+    if (L == 32) return (threadIdx.x & 32) ? read_lane(v, 63) : read_lane(v, 31);
+    if (L == 64) return read_lane(v, 63);
     return v;
 }
 
