@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdlib>
+#include <type_traits>
 
 #include "fnet_vec.h"
 
@@ -11,7 +12,7 @@ namespace {
 constexpr int kThreads = 256;
 // Every launch carries its part of the list as a kernel argument (below 4 KB): nothing is uploaded, so there is no table whose lifetime a
 // captured graph or another stream could outlive.
-constexpr int kTab = 240, kAdamTab = 80;
+constexpr int kTab = 240, kAdamTab = 96, kMasterTab = 80;
 constexpr long long kMaxEntry = 1ll << 30;       // a longer tensor takes several entries
 constexpr int kMaxBlocks = 2048;                 // eight blocks of four waves per CU; also the number of partial sums every consumer re-reads
 
@@ -24,13 +25,25 @@ struct ListTab {
     int count;
     uint32_t chunks;
 };
-struct AdamTab {
-    uint64_t p[kAdamTab], g[kAdamTab], m[kAdamTab], v[kAdamTab], w[kAdamTab];
+struct AdamTab {                  // of fp32 parameters, which are their own masters
+    uint64_t p[kAdamTab], g[kAdamTab], m[kAdamTab], v[kAdamTab];
     uint32_t n[kAdamTab], first[kAdamTab];
     int count;
     uint32_t chunks;
+    static constexpr int SIZE = kAdamTab;
+    __host__ __device__ uint64_t& master(int j) { return p[j]; }
+    __host__ __device__ uint64_t master(int j) const { return p[j]; }
 };
-static_assert(sizeof(ListTab) <= 3904 && sizeof(AdamTab) <= 3904, "the table and the other arguments must fit 4 KB");
+struct MasterTab {
+    uint64_t p[kMasterTab], g[kMasterTab], m[kMasterTab], v[kMasterTab], w[kMasterTab];
+    uint32_t n[kMasterTab], first[kMasterTab];
+    int count;
+    uint32_t chunks;
+    static constexpr int SIZE = kMasterTab;
+    __host__ __device__ uint64_t& master(int j) { return w[j]; }
+    __host__ __device__ uint64_t master(int j) const { return w[j]; }
+};
+static_assert(sizeof(ListTab) <= 3904 && sizeof(AdamTab) <= 3904 && sizeof(MasterTab) <= 3904, "the table and the other arguments must fit 4 KB");
 
 // the entry that chunk c belongs to: every lane looks at one entry, 64 per step (a scan by one lane would be a chain of dependent loads)
 template <typename TAB>
@@ -272,9 +285,10 @@ __device__ __forceinline__ void store8(T* p, const float* v) {
     if (VecOf<T>::V == 4) store_chunk<T>(p + 4, 4, v + (VecOf<T>::V == 4 ? 4 : 0));
 }
 
-// MASTER: w is a buffer of its own and p (type T) its rounding; otherwise T is float and p is the weight
-template <typename T, bool MASTER>
-__global__ __launch_bounds__(256) void k_list_adam(AdamTab t, AdamArgs a) {
+// MasterTab: w is a buffer of its own and p (type T) its rounding; otherwise T is float and p is the weight
+template <typename T, typename TAB>
+__global__ __launch_bounds__(256) void k_list_adam(TAB t, AdamArgs a) {
+    constexpr bool MASTER = !std::is_same<TAB, AdamTab>::value;
     __shared__ double red[4];
     AdamCoef k;
     k.coef = a.clip ? coef_of(a.f, red) : 1.f;
@@ -290,7 +304,7 @@ __global__ __launch_bounds__(256) void k_list_adam(AdamTab t, AdamArgs a) {
         const T* G = gptr<const T>(t.g[j]);
         T* P = gptr<T>(t.p[j]);
         float *M = gptr<float>(t.m[j]), *S = gptr<float>(t.v[j]);
-        float* W = MASTER ? gptr<float>(t.w[j]) : gptr<float>(t.p[j]);
+        float* W = gptr<float>(t.master(j));
 #pragma unroll
         for (int q = 0; q < kAdamVecs; ++q) {
             const uint32_t o = at + (q * kThreads + threadIdx.x) * 8;
@@ -546,38 +560,42 @@ int fnet_list_adam(int32_t n, const uint64_t* host_param, const uint64_t* host_g
     a.omb2 = (float)(1.0 - h->beta2);
     a.eps = (float)h->eps;
     hipStream_t st = (hipStream_t)stream;
-    auto flush = [&](int d, AdamTab& t) -> int {
-        const dim3 grid(std::min<uint32_t>(t.chunks, kMaxBlocks));
-        if (d == FNET_F32) hipLaunchKernelGGL((k_list_adam<float, false>), grid, dim3(kThreads), 0, st, t, a);
-        else if (d == FNET_BF16) hipLaunchKernelGGL((k_list_adam<bf16_t, true>), grid, dim3(kThreads), 0, st, t, a);
-        else hipLaunchKernelGGL((k_list_adam<f16_t, true>), grid, dim3(kThreads), 0, st, t, a);
-        FNET_LAUNCH_CHECK();
-        a.f.norm_out = nullptr;
-        t.count = 0;
-        t.chunks = 0;
-        return FNET_OK;
-    };
-    for (int d = 0; d <= FNET_F16; ++d) {
-        AdamTab t;
-        t.count = 0;
-        t.chunks = 0;
-        for (int k = 0; k < n; ++k) {
-            if (host_dtype[k] != d) continue;
-            for (int64_t at = 0; at < host_numel[k]; at += kMaxEntry) {
-                const uint32_t len = (uint32_t)std::min<int64_t>(host_numel[k] - at, kMaxEntry);
-                const int i = t.count;
-                t.p[i] = host_param[k] + (uint64_t)at * elem_size(d);
-                t.g[i] = host_grad[k] + (uint64_t)at * elem_size(d);
-                t.m[i] = host_exp_avg[k] + (uint64_t)at * 4;
-                t.v[i] = host_exp_avg_sq[k] + (uint64_t)at * 4;
-                t.w[i] = d == FNET_F32 ? 0 : host_master[k] + (uint64_t)at * 4;
-                t.n[i] = len;
-                t.first[i] = t.chunks;
-                t.chunks += (len + kAdamChunk - 1) / kAdamChunk;
-                if (++t.count == kAdamTab && (rc = flush(d, t)) != FNET_OK) return rc;
+    for (int d = 0; d <= FNET_F16 && rc == FNET_OK; ++d) {
+        auto run = [&](auto t, auto kernel) -> int {
+            t.count = 0;
+            t.chunks = 0;
+            auto flush = [&]() -> int {
+                hipLaunchKernelGGL(kernel, dim3(std::min<uint32_t>(t.chunks, kMaxBlocks)), dim3(kThreads), 0, st, t, a);
+                FNET_LAUNCH_CHECK();
+                a.f.norm_out = nullptr;
+                t.count = 0;
+                t.chunks = 0;
+                return FNET_OK;
+            };
+            for (int k = 0; k < n; ++k) {
+                if (host_dtype[k] != d) continue;
+                for (int64_t at = 0; at < host_numel[k]; at += kMaxEntry) {
+                    const uint32_t len = (uint32_t)std::min<int64_t>(host_numel[k] - at, kMaxEntry);
+                    const int i = t.count;
+                    t.p[i] = host_param[k] + (uint64_t)at * elem_size(d);
+                    t.g[i] = host_grad[k] + (uint64_t)at * elem_size(d);
+                    t.m[i] = host_exp_avg[k] + (uint64_t)at * 4;
+                    t.v[i] = host_exp_avg_sq[k] + (uint64_t)at * 4;
+                    t.master(i) = (d == FNET_F32 ? host_param[k] : host_master[k]) + (uint64_t)at * 4;
+                    t.n[i] = len;
+                    t.first[i] = t.chunks;
+                    t.chunks += (len + kAdamChunk - 1) / kAdamChunk;
+                    if (++t.count == t.SIZE) {
+                        const int e = flush();
+                        if (e != FNET_OK) return e;
+                    }
+                }
             }
-        }
-        if (t.count && (rc = flush(d, t)) != FNET_OK) return rc;
+            return t.count ? flush() : FNET_OK;
+        };
+        if (d == FNET_F32) rc = run(AdamTab(), k_list_adam<float, AdamTab>);
+        else if (d == FNET_BF16) rc = run(MasterTab(), k_list_adam<bf16_t, MasterTab>);
+        else rc = run(MasterTab(), k_list_adam<f16_t, MasterTab>);
     }
-    return FNET_OK;
+    return rc;
 }

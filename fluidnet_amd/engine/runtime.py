@@ -145,14 +145,21 @@ def current_stream_ptr() -> int:
 def call_on(t, name: str, *args) -> None:
     """An entry point whose last argument is the stream, on the current stream of the device that tensor `t` lies on."""
     import torch
-    fn, dev = getattr(lib(), name), t.device
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    fn, dev = getattr(lib(), name), t.get_device()
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = fn(*args, _raw_stream(dev))
     if rc:
         check(rc, name)
+
+
+def _raw_stream(dev: int) -> int:
+    """cudaStream_t of device dev's current stream: a fifteenth of the time that torch.cuda.current_stream(dev).cuda_stream takes, on calls
+    that take a few microseconds altogether."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def run_ops(ops: np.ndarray, stream: Optional[int] = None) -> None:

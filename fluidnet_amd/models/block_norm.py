@@ -23,7 +23,6 @@ There is no CPU fallback.
 """
 from __future__ import annotations
 
-import ctypes
 import struct
 from typing import Literal, Optional, Tuple
 
@@ -46,15 +45,15 @@ _ARGS = struct.Struct("=7q8i2f22Qq")
 
 class _Spec:
     """What a call is, apart from its tensors."""
-    __slots__ = ("rows", "tokens", "width", "dtype", "param_dtype", "gate_dtype", "kind", "post", "pre", "gate_kind", "gate_act",
-                 "residual_scale", "eps")
+    __slots__ = ("rows", "tokens", "width", "param_dtype", "gate_dtype", "pre", "post", "gate_kind", "samples", "fixed")
 
 
 def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     """The tensor (copied if its last axis is not dense or its rows are not evenly spaced) and its row stride."""
+    size = t.shape
     if t.is_contiguous():
-        return t, t.shape[-1]
-    size, stride = t.shape, t.stride()
+        return t, size[-1]
+    stride = t.stride()
     if stride[-1] == 1 or size[-1] == 1:
         step, n = None, 1                     # distance of neighbouring rows, rows in the axes looked at so far
         for d in range(t.ndim - 2, -1, -1):
@@ -70,10 +69,8 @@ def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     return t.contiguous(), size[-1]
 
 
-def _param_type(name: str, t: Optional[torch.Tensor], C: int, x: torch.Tensor, seen):
-    if t is None:
-        return seen
-    if t.shape != (C,) or t.device != x.device:
+def _param_type(name: str, t: torch.Tensor, C: int, x: torch.Tensor, seen):
+    if t.shape != (C,) or t.get_device() != x.get_device():
         raise ValueError(f"{name} must have shape ({C},) on {x.device} (got {tuple(t.shape)} on {t.device})")
     if t.dtype is not torch.float32 and t.dtype is not x.dtype:
         raise ValueError(f"{name} must be float32 or {x.dtype} (got {t.dtype})")
@@ -103,78 +100,117 @@ def _spec(x, branch, gate, scale, pw, pb, nw, nb, kind, post, pre, gate_act, res
     code = ELEM.get(x.dtype)
     if code is None:
         raise ValueError(f"x must be float32, bfloat16 or float16 (got {x.dtype})")
-    if x.ndim < 1 or not 1 <= x.shape[-1] <= MAX_WIDTH:
-        raise ValueError(f"the last axis must have 1 to {MAX_WIDTH} elements (got shape {tuple(x.shape)})")
+    shape = x.shape
+    if not shape or not 1 <= shape[-1] <= MAX_WIDTH:
+        raise ValueError(f"the last axis must have 1 to {MAX_WIDTH} elements (got shape {tuple(shape)})")
     if kind not in _KIND or gate_act not in _ACT:
         raise ValueError(f"kind must be one of {tuple(_KIND)} and gate_act one of {tuple(_ACT)} (got {kind!r}, {gate_act!r})")
     if not eps >= 0:
         raise ValueError(f"eps must not be negative (got {eps})")
-    C = x.shape[-1]
     s = _Spec()
-    s.width, s.dtype = C, code
-    s.rows = x.numel() // C
-    if s.rows >= 1 << 31:
+    s.width = C = shape[-1]
+    s.rows = rows = x.numel() // C
+    if rows >= 1 << 31:
         raise ValueError("at most 2^31 - 1 rows")
-    s.tokens = s.rows // x.shape[0] if x.ndim > 1 and x.shape[0] else s.rows
     if branch is None:
         if gate is not None or scale is not None:
             raise ValueError("a gate or scale needs a branch")
         post = False
-    else:
-        if branch.shape != x.shape or branch.dtype is not x.dtype or branch.device != x.device:
-            raise ValueError(f"branch must be like x: {tuple(x.shape)} {x.dtype} on {x.device} (got {tuple(branch.shape)} {branch.dtype} on {branch.device})")
+    elif branch.shape != shape or branch.dtype is not x.dtype or branch.get_device() != x.get_device():
+        raise ValueError(f"branch must be like x: {tuple(shape)} {x.dtype} on {x.device} (got {tuple(branch.shape)} {branch.dtype} on {branch.device})")
     if not post and (pw is not None or pb is not None):
         raise ValueError("post_weight / post_bias need post=True")
     if not pre and (nw is not None or nb is not None):
         raise ValueError("pre_weight / pre_bias need pre=True")
     seen = None
-    for name, t in (("scale", scale), ("post_weight", pw), ("post_bias", pb), ("pre_weight", nw), ("pre_bias", nb)):
-        seen = _param_type(name, t, C, x, seen)
-    s.param_dtype = 0 if seen is None else ELEM[seen]
-    s.gate_kind, s.gate_dtype = _NONE, 0
+    if scale is not None:
+        seen = _param_type("scale", scale, C, x, seen)
+    if pw is not None:
+        seen = _param_type("post_weight", pw, C, x, seen)
+    if pb is not None:
+        seen = _param_type("post_bias", pb, C, x, seen)
+    if nw is not None:
+        seen = _param_type("pre_weight", nw, C, x, seen)
+    if nb is not None:
+        seen = _param_type("pre_bias", nb, C, x, seen)
+    gate_kind, gate_dtype, s.tokens, s.samples = _NONE, 0, rows, 1
     if gate is not None:
-        if gate.device != x.device or (gate.dtype is not torch.float32 and gate.dtype is not x.dtype):
+        if gate.get_device() != x.get_device() or (gate.dtype is not torch.float32 and gate.dtype is not x.dtype):
             raise ValueError(f"gate must be float32 or {x.dtype} on {x.device} (got {gate.dtype} on {gate.device})")
-        s.gate_kind, s.gate_dtype = _gate_kind(gate, x), ELEM[gate.dtype]
-    s.kind, s.post, s.pre, s.gate_act = _KIND[kind], bool(post), bool(pre), _ACT[gate_act]
-    s.residual_scale, s.eps = float(residual_scale), float(eps)
+        gate_kind, gate_dtype = _gate_kind(gate, x), ELEM[gate.dtype]
+        if gate_kind == _SAMPLE and rows:
+            s.samples = shape[0]
+            s.tokens = rows // s.samples
+            if s.tokens == 1:                 # a row of values per row
+                gate_kind = _ELEMENT
+    s.gate_kind, s.pre, s.post = gate_kind, bool(pre), bool(post)
+    s.fixed = (C, code, 0 if seen is None else ELEM[seen], gate_dtype, _KIND[kind], s.post, gate_kind, _ACT[gate_act], float(residual_scale), float(eps))
     if not x.is_cuda:
         raise RuntimeError("fluidnet_amd block norms run on MI355X only (got a CPU tensor); there is no CPU fallback")
     return s
 
 
-def _gate_rows(s: _Spec, gate: Optional[torch.Tensor]) -> Tuple[Optional[torch.Tensor], int]:
+def _gate_rows(s: _Spec, gate: torch.Tensor) -> Tuple[torch.Tensor, int]:
     """The gate and the distance of its rows (of its values, for one per token)."""
-    if gate is None:
-        return None, 0
-    if s.gate_kind in (_ELEMENT, _TOKEN):
+    if s.gate_kind == _ELEMENT or s.gate_kind == _TOKEN:
         return _rows(gate)
     if s.gate_kind == _SAMPLE and gate.stride(-1) == 1:
         return gate, gate.stride(0)
     return gate.contiguous(), s.width
 
 
-def _ptr(t: Optional[torch.Tensor]) -> int:
-    return 0 if t is None else t.data_ptr()
+def _operands(s: _Spec, x, branch, gate, scale, pw, pb, nw, nb):
+    """What the kernels read besides gradients, as they take it: strides, addresses and the tensors these belong to."""
+    x, xs = _rows(x)
+    b = g = c = d = e = f = h = bs = gs = 0
+    if branch is not None:
+        branch, bs = _rows(branch)
+        b = branch.data_ptr()
+        if gate is not None:
+            gate, gs = _gate_rows(s, gate)
+            g = gate.data_ptr()
+        if scale is not None:
+            scale = scale.contiguous()
+            c = scale.data_ptr()
+        if pw is not None:
+            pw = pw.contiguous()
+            d = pw.data_ptr()
+        if pb is not None:
+            pb = pb.contiguous()
+            e = pb.data_ptr()
+    if nw is not None:
+        nw = nw.contiguous()
+        f = nw.data_ptr()
+    if nb is not None:
+        nb = nb.contiguous()
+        h = nb.data_ptr()
+    return (xs, bs, gs), (x.data_ptr(), b, g, c, d, e, f, h), (x, branch, gate, scale, pw, pb, nw, nb)
 
 
-def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return t if t is None or t.is_contiguous() else t.contiguous()
+_NO_GRADS = (0,) * 12
+_DENSE = torch.contiguous_format
 
 
 def _forward(s: _Spec, x, branch, gate, scale, pw, pb, nw, nb, keep: bool):
-    """(y, h, stats) of prepared operands."""
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if branch is not None else None
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if s.pre else None
-    stats = torch.empty((4, s.rows), dtype=torch.float32, device=x.device) if keep and (s.post or s.pre) else None
+    """(y, h, stats): stats (means and deviations, for the backward) if they are kept."""
+    y = torch.empty_like(x, memory_format=_DENSE) if branch is not None else None
+    h = torch.empty_like(x, memory_format=_DENSE) if s.pre else None
+    stats = x.new_empty((4, s.rows), dtype=torch.float32) if keep and (s.post or s.pre) else None
     if s.rows and (y is not None or h is not None):
-        (xt, xs), (bt, bs), (gt, gs) = _rows(x), (_rows(branch) if branch is not None else (None, 0)), _gate_rows(s, gate)
-        params = [_dense(t) for t in (scale, pw, pb, nw, nb)]
-        a = _ARGS.pack(s.rows, s.tokens, xs, bs, gs, 0, 0, s.width, s.dtype, s.param_dtype, s.gate_dtype, s.kind, s.post, s.gate_kind, s.gate_act,
-                       s.residual_scale, s.eps, xt.data_ptr(), _ptr(bt), _ptr(gt), *map(_ptr, params), _ptr(y), _ptr(h), _ptr(stats),
-                       0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+        strides, ptrs, _keep = _operands(s, x, branch, gate, scale, pw, pb, nw, nb)
+        a = _ARGS.pack(s.rows, s.tokens, *strides, 0, 0, *s.fixed, *ptrs, 0 if y is None else y.data_ptr(), 0 if h is None else h.data_ptr(),
+                       0 if stats is None else stats.data_ptr(), *_NO_GRADS)
         rt.call_on(x, "fnet_block_norm_fwd", a)
     return y, h, stats
+
+
+def _workspace(s: _Spec, sums: int) -> int:
+    """Bytes that hold the partial sums of a backward with so many gradients over rows (fnet_block_norm_workspace gives the exact number): at
+    most a row per four rows of the operands, and per block that fits the GPU or sample."""
+    C = s.width
+    blocks = 1024 if C <= 2048 else 256 * max(1, 16 // -(-C // 512))
+    rows = min(s.rows, max(blocks, s.samples))
+    return sums * (4 * C * rows + 16)
 
 
 class _BlockNormFn(torch.autograd.Function):
@@ -190,41 +226,55 @@ class _BlockNormFn(torch.autograd.Function):
     def backward(ctx, dy, dh):
         s = ctx.s
         x, branch, gate, scale, pw, pb, nw, nb, stats = ctx.saved_tensors
-        none = (None,) * 9
-        if dy is None and dh is None:
-            return none
         _, nx, nbr, ng, nsc, npw, npb, nnw, nnb = ctx.needs_input_grad
-        new = lambda t, need: torch.empty(t.shape, dtype=t.dtype, device=t.device) if need and t is not None else None  # noqa: E731
-        if s.rows == 0:
-            return (None, *(None if not n or t is None else torch.zeros(t.shape, dtype=t.dtype, device=t.device) for t, n in
-                            zip((x, branch, gate, scale, pw, pb, nw, nb), ctx.needs_input_grad[1:])))
+        if dy is None and dh is None:
+            return (None,) * 9
+        make = torch.empty_like if s.rows else torch.zeros_like
+        with_h = dh is not None
         # without a gradient of h, the gradient of x is that of y
-        dx = (dy if dh is None else new(x, True)) if nx else None
-        db, dg, dsc, dpw, dpb = new(branch, nbr), new(gate, ng), new(scale, nsc), new(pw, npw), new(pb, npb)
-        zero = lambda t, need: torch.zeros(t.shape, dtype=t.dtype, device=t.device) if need and t is not None else None  # noqa: E731
-        dnw, dnb = (new(nw, nnw), new(nb, nnb)) if dh is not None else (zero(nw, nnw), zero(nb, nnb))
-        if (dh is not None and (nx or nnw or nnb)) or any(t is not None for t in (db, dg, dsc, dpw, dpb)):
-            (xt, xs), (bt, bs), (gt, gs) = _rows(x), (_rows(branch) if branch is not None else (None, 0)), _gate_rows(s, gate)
-            (dyt, dys), (dht, dhs) = (_rows(t) if t is not None else (None, 0) for t in (dy, dh))
-            params = [_dense(t) for t in (scale, pw, pb, nw, nb)]
-            with_dh = dh is not None
-
-            def pack(ws, n):
-                return _ARGS.pack(s.rows, s.tokens, xs, bs, gs, dys, dhs, s.width, s.dtype, s.param_dtype, s.gate_dtype, s.kind, s.post,
-                                  s.gate_kind, s.gate_act, s.residual_scale, s.eps, xt.data_ptr(), _ptr(bt), _ptr(gt), *map(_ptr, params), 0, 0,
-                                  _ptr(stats), _ptr(dyt), _ptr(dht), _ptr(dx) if with_dh else 0, _ptr(db), _ptr(dg), _ptr(dsc), _ptr(dpw),
-                                  _ptr(dpb), _ptr(dnw) if with_dh else 0, _ptr(dnb) if with_dh else 0, ws, n)
-            need = ctypes.c_int64()
-            rt.check(rt.lib().fnet_block_norm_workspace(pack(0, 0), ctypes.byref(need)), "fnet_block_norm_workspace")
-            ws = torch.empty(need.value, dtype=torch.uint8, device=x.device) if need.value else None
-            rt.call_on(x, "fnet_block_norm_bwd", pack(_ptr(ws), need.value))
+        dx = None if not nx else make(x, memory_format=_DENSE) if with_h else dy
+        db = make(branch, memory_format=_DENSE) if nbr and branch is not None else None
+        dg = make(gate, memory_format=_DENSE) if ng and gate is not None else None
+        sums = 0 if dg is None else 1
+        dsc = dpw = dpb = dnw = dnb = None
+        if nsc and scale is not None:
+            dsc, sums = make(scale, memory_format=_DENSE), sums + 1
+        if npw and pw is not None:
+            dpw, sums = make(pw, memory_format=_DENSE), sums + 1
+        if npb and pb is not None:
+            dpb, sums = make(pb, memory_format=_DENSE), sums + 1
+        norm = make if with_h else torch.zeros_like
+        if nnw and nw is not None:
+            dnw, sums = norm(nw, memory_format=_DENSE), sums + 1
+        if nnb and nb is not None:
+            dnb, sums = norm(nb, memory_format=_DENSE), sums + 1
+        if s.rows and (with_h or db is not None or dg is not None or sums):
+            strides, ptrs, _keep = _operands(s, x, branch, gate, scale, pw, pb, nw, nb)
+            py = ys = ph = hs = px = p0 = p1 = 0
+            if dy is not None:
+                dy, ys = _rows(dy)
+                py = dy.data_ptr()
+            if with_h:
+                dh, hs = _rows(dh)
+                ph = dh.data_ptr()
+                px = 0 if dx is None else dx.data_ptr()
+                p0 = 0 if dnw is None else dnw.data_ptr()
+                p1 = 0 if dnb is None else dnb.data_ptr()
+            n = _workspace(s, sums) if sums else 0
+            ws = x.new_empty(n, dtype=torch.uint8) if n else None
+            a = _ARGS.pack(s.rows, s.tokens, *strides, ys, hs, *s.fixed, *ptrs, 0, 0, 0 if stats is None else stats.data_ptr(), py, ph, px,
+                           0 if db is None else db.data_ptr(), 0 if dg is None else dg.data_ptr(), 0 if dsc is None else dsc.data_ptr(),
+                           0 if dpw is None else dpw.data_ptr(), 0 if dpb is None else dpb.data_ptr(), p0, p1, 0 if ws is None else ws.data_ptr(), n)
+            rt.call_on(x, "fnet_block_norm_bwd", a)
         return None, dx, db, dg, dsc, dpw, dpb, dnw, dnb
 
 
-def _run(s: _Spec, x, branch, gate, scale, pw, pb, nw, nb):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, branch, gate, scale, pw, pb, nw, nb)):
-        return _BlockNormFn.apply(s, x, branch, gate, scale, pw, pb, nw, nb)
-    y, h, _ = _forward(s, x, branch, gate, scale, pw, pb, nw, nb, False)
+def _run(s: _Spec, *operands):
+    if torch.is_grad_enabled():
+        for t in operands:
+            if t is not None and t.requires_grad:
+                return _BlockNormFn.apply(s, *operands)
+    y, h, _ = _forward(s, *operands, False)
     return y, h
 
 

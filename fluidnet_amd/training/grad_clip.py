@@ -14,6 +14,7 @@ import ctypes
 import math
 import struct
 from array import array
+from operator import attrgetter
 from typing import Iterable, List, Union
 
 import torch
@@ -44,37 +45,48 @@ def _collapsed(t: torch.Tensor):
     return out
 
 
+# Over hundreds of tensors the checks cost more than the kernels: each is one pass of C code over the list, and only a list that fails one is
+# looked at tensor by tensor.
+_device, _contiguous, _numel, _address = (getattr(torch.Tensor, n) for n in ("get_device", "is_contiguous", "numel", "data_ptr"))
+_dtype, _shape = attrgetter("dtype"), attrgetter("shape")
+
+
 class TensorList:
     """Addresses, element counts and types of the tensors of a call, as the C ABI takes them.  Lives for the call only."""
 
     def __init__(self, tensors: List[torch.Tensor], what: str = "gradient") -> None:
-        device = tensors[0].get_device()
+        self.first = tensors[0]
+        device = self.first.get_device()
         if device < 0:
             raise RuntimeError(f"fluidnet_amd runs on MI355X only (got a CPU {what}); there is no CPU fallback")
-        self.first = tensors[0]
-        ptrs, numels, codes, strided = [], [], [], []
-        for k, t in enumerate(tensors):
-            code = ELEM.get(t.dtype)
-            if code is None or t.get_device() != device or t.layout is not torch.strided:
-                raise ValueError(f"{what} {k} must be a dense float32, bfloat16 or float16 tensor on {tensors[0].device} "
-                                 f"(got {t.dtype}, {t.layout}, {t.device})")
-            if not t.is_contiguous():
-                axes = _collapsed(t)
-                if axes is None or len(axes) > _MAXDIM:
-                    raise ValueError(f"{what} {k}: elements that share memory, or more than {_MAXDIM} separate axes (shape {tuple(t.shape)}, "
-                                     f"strides {t.stride()})")
-                if len(axes) > 1 or (axes and axes[0][0] != 1):
-                    pad = [0] * (_MAXDIM - len(axes))
-                    strided.append(_STRIDED.pack(t.data_ptr(), code, len(axes), *(n for _, n in axes), *pad, *(st for st, _ in axes), *pad))
-                    continue
-            ptrs.append(t.data_ptr())
-            numels.append(t.numel())
-            codes.append(code)
-        self.n, self.n_strided = len(ptrs), len(strided)
-        self._keep = (array("Q", ptrs), array("q", numels), array("i", codes), b"".join(strided))
+        types = list(map(_dtype, tensors))
+        if not (ELEM.keys() >= set(types) and set(map(_device, tensors)) == {device}):
+            k, t = next((k, t) for k, t in enumerate(tensors) if t.dtype not in ELEM or t.get_device() != device)
+            raise ValueError(f"{what} {k} must be a float32, bfloat16 or float16 tensor on {self.first.device} (got {t.dtype} on {t.device})")
+        strided = []
+        if not all(map(_contiguous, tensors)):
+            tensors, types, strided = self._split(tensors, what)
+        self.n, self.n_strided = len(tensors), len(strided)
+        self._keep = (array("Q", map(_address, tensors)), array("q", map(_numel, tensors)), array("i", map(ELEM.__getitem__, types)), b"".join(strided))
         self.ptrs, self.numels, self.codes = (a.buffer_info()[0] for a in self._keep[:3])
         self.strided = ctypes.cast(ctypes.c_char_p(self._keep[3]), ctypes.c_void_p) if strided else None
         self.capacity = 2048 + self.n // 64 + 256 * self.n_strided + 8
+
+    @staticmethod
+    def _split(tensors, what):
+        """The dense tensors, their types, and the records of those that are no dense block of memory."""
+        dense, strided = [], []
+        for k, t in enumerate(tensors):
+            axes = [[1, t.numel()]] if t.is_contiguous() else _collapsed(t)
+            if axes is None or len(axes) > _MAXDIM:
+                raise ValueError(f"{what} {k}: elements that share memory, or more than {_MAXDIM} separate axes (shape {tuple(t.shape)}, "
+                                 f"strides {t.stride()})")
+            if len(axes) > 1 or (axes and axes[0][0] != 1):
+                pad = [0] * (_MAXDIM - len(axes))
+                strided.append(_STRIDED.pack(t.data_ptr(), ELEM[t.dtype], len(axes), *(n for _, n in axes), *pad, *(st for st, _ in axes), *pad))
+            else:
+                dense.append(t)
+        return dense, [t.dtype for t in dense], strided
 
     def args(self):
         return self.n, self.ptrs, self.numels, self.codes, self.n_strided, self.strided
@@ -113,7 +125,6 @@ def _grads(parameters) -> List[torch.Tensor]:
     return [g for g in [p.grad for p in parameters] if g is not None]
 
 
-@torch.no_grad()
 def total_grad_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0) -> torch.Tensor:
     """The norm of all elements of `tensors` (gradients, or anything else), a 0-dim fp32 tensor on their device.  0 for an empty list, on
     the CPU (as torch.nn.utils.get_total_norm)."""
@@ -126,7 +137,6 @@ def _scale(lst: TensorList, max_norm: float, kind: int, partials: int, used: int
     rt.call_on(lst.first, "fnet_list_scale", *lst.args(), partials, used, kind, norm, max_norm, out)
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """Scales the gradients of `parameters` in place by min(1, max_norm / (norm + 1e-6)) and returns the norm that they had (0-dim, fp32, on
@@ -152,7 +162,6 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     return total
 
 
-@torch.no_grad()
 def clip_grads_with_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, total_norm: torch.Tensor) -> None:
     """The scaling alone, by a norm that is known: one element, on the gradients' device (for instance a norm reduced over ranks)."""
     max_norm = _max_norm(max_norm)

@@ -17,7 +17,7 @@ import torch
 
 from ..engine import runtime as rt
 from ..engine.runtime import OPC
-from .grad_clip import TensorList, _collapsed, _max_norm
+from .grad_clip import TensorList, _address, _collapsed, _contiguous, _device, _dtype, _max_norm, _numel, _shape
 
 
 class FusedClipAdam:
@@ -93,7 +93,17 @@ def _same_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
 _ADAM = struct.Struct("=6d4Qi4x")
 
 
-@torch.no_grad()
+def _check_layouts(params, grads, exp_avgs, exp_avg_sqs, masters) -> None:
+    """Tensor by tensor what clip_adam_ asks of a whole list: raises for the first one that does not fit; dense tensors in another order pass."""
+    for k, (p, g, m, v, w) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs, masters)):
+        if p.dtype is not g.dtype or p.get_device() != g.get_device() or not _same_layout(p, g):
+            raise ValueError(f"parameter {k} and its gradient must be dense tensors of one type, layout and device (got "
+                             f"{tuple(p.shape)} {p.stride()} {p.dtype} {p.device}, {tuple(g.shape)} {g.stride()} {g.dtype} {g.device})")
+        for name, t in (("exp_avg", m), ("exp_avg_sq", v)) + ((("master", w),) if p.dtype is not torch.float32 else ()):
+            if t.dtype is not torch.float32 or t.get_device() != p.get_device() or not _same_layout(p, t):
+                raise ValueError(f"{name} {k} must be a float32 tensor laid out like its parameter: {tuple(p.shape)} {p.stride()} on {p.device}")
+
+
 def clip_adam_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
                exp_avg_sqs: Sequence[torch.Tensor], clock: torch.Tensor, *, masters: Optional[Sequence[torch.Tensor]] = None,
                lr: Union[float, torch.Tensor], betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.0,
@@ -120,22 +130,25 @@ def clip_adam_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         max_norm = _max_norm(max_norm)
     lst = TensorList(grads)
     dev, f32 = lst.first.get_device(), torch.float32
-    for k in range(n):
-        p, g, m, v, w = params[k], grads[k], exp_avgs[k], exp_avg_sqs[k], masters[k]
-        if p.dtype is not g.dtype or p.get_device() != dev or not _same_layout(p, g):
-            raise ValueError(f"parameter {k} and its gradient must be dense tensors of one type, layout and device (got "
-                             f"{tuple(p.shape)} {p.stride()} {p.dtype} {p.device}, {tuple(g.shape)} {g.stride()} {g.dtype} {g.device})")
-        low = p.dtype is not f32
-        if low and w is None:
-            raise ValueError(f"parameter {k} is {p.dtype} and needs an fp32 master")
-        for name, t in (("exp_avg", m), ("exp_avg_sq", v)) + ((("master", w),) if low else ()):
-            if t.dtype is not f32 or t.get_device() != dev or not _same_layout(p, t):
-                raise ValueError(f"{name} {k} must be a float32 tensor laid out like its parameter: {tuple(p.shape)} {p.stride()} on {p.device}")
+    types = list(map(_dtype, params))
+    low = [k for k, t in enumerate(types) if t is not f32]
+    if any(masters[k] is None for k in low):
+        raise ValueError(f"parameter {next(k for k in low if masters[k] is None)} is not float32 and needs an fp32 master")
+    state = exp_avgs + exp_avg_sqs + [masters[k] for k in low]
+    numels = list(map(_numel, grads))
+    if not (types == list(map(_dtype, grads)) and set(map(_dtype, state)) == {f32} and set(map(_device, params + state)) == {dev}
+            and list(map(_shape, params)) == list(map(_shape, grads)) and list(map(_numel, state)) == numels + numels + [numels[k] for k in low]
+            and all(map(_contiguous, params + grads + state))):
+        _check_layouts(params, grads, exp_avgs, exp_avg_sqs, masters)
     for name, t, count in (("clock", clock, 3),) + ((("lr", lr, 1),) if isinstance(lr, torch.Tensor) else ()):
         if t.dtype is not torch.float64 or t.numel() != count or t.get_device() != dev or not t.is_contiguous():
             raise ValueError(f"{name} must be {count} float64 value(s) on {lst.first.device}")
-    ptrs = [array("Q", [0 if t is None else t.data_ptr() for t in ts]) for ts in (params, exp_avgs, exp_avg_sqs, masters)]
-    address = [a.buffer_info()[0] for a in ptrs]
+    ptrs = [array("Q", map(_address, ts)) for ts in (params, exp_avgs, exp_avg_sqs)]
+    if low:
+        ptrs.append(array("Q", [0] * n))
+        for k in low:
+            ptrs[3][k] = masters[k].data_ptr()
+    address = [a.buffer_info()[0] for a in ptrs] + [None] * (4 - len(ptrs))
     total, partials, used = None, None, 0
     if max_norm is not None:
         total = torch.empty((), dtype=f32, device=lst.first.device)
