@@ -16,9 +16,10 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libfluidnet_hip.so")
 SOURCES = ["fnet_elementwise.hip", "fnet_loss.hip", "fnet_conv_ref.hip", "fnet_conv_mfma.hip", "fnet_optim.hip", "fnet_plan.hip", "fnet_rollout.hip",
-           "fnet_block_norm.hip", "fnet_block_norm_bwd.hip", "fnet_block_norm_bwd_f32.hip", "fnet_block_norm_bwd_bf16.hip",
-           "fnet_block_norm_bwd_f16.hip", "fnet_tensor_list.hip"]
-HEADERS = [os.path.join(CSRC, h) for h in ("fnet_common.h", "fnet_vec.h", "fnet_block_norm.h", "fnet_block_norm_bwd.h")] + [os.path.join(os.path.dirname(HERE), "include", "fluidnet_hip.h")]
+           "fnet_block_norm.hip", "fnet_block_norm_f32.hip", "fnet_block_norm_bf16.hip", "fnet_block_norm_f16.hip",
+           "fnet_tensor_list.hip"]
+HEADERS = [os.path.join(CSRC, h) for h in ("fnet_common.h", "fnet_vec.h", "fnet_block_norm.h", "fnet_block_norm_fwd.h",
+                                             "fnet_block_norm_bwd.h")] + [os.path.join(os.path.dirname(HERE), "include", "fluidnet_hip.h")]
 # -packed-fp32-ops: hipcc makes v_pk_{add,mul,fma}_f32 of ordinary float code by itself, and some of their forms have given wrong results on
 # MI355X now and then; the scalar forms are as fast for code that memory bounds.  (The host pass warns that it does not know the feature.)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-ffp-contract=off", "-Wall", "-Wno-unused-function", "-Wno-unused-value",

@@ -83,6 +83,46 @@ struct RowSum {
     }
 };
 
+// Mean and sum of squares about it of a row, for several waves to a row behind ONE barrier: each wave takes its own mean and its squares about
+// that, and the waves' are joined as n_w (mean_w - mean)^2 + squares_w.  No difference of large numbers anywhere.  n: elements of wave
+// (threadIdx.x & 15) of this row.  `red` as RowSum<L, 2>.
+template <int L>
+struct RowMoments {
+    RowSum<L, 2>& sum;
+    float inv_c, n_wave, inv_wave, n;
+    __device__ __forceinline__ RowMoments(RowSum<L, 2>& s, const RowPlace<L>& at, int width, int V, int K) : sum(s), inv_c(1.f / (float)width) {
+        auto elements = [&](int wave) {
+            int c = 0;
+            for (int k = 0; k < K; ++k) c += min(max(width - (k * at.lanes + 64 * wave) * V, 0), 64 * V);
+            return (float)c;
+        };
+        n_wave = elements(at.lane >> 6);
+        inv_wave = n_wave > 0.f ? 1.f / n_wave : 0.f;
+        n = (int)(threadIdx.x & 15) < at.waves ? elements(threadIdx.x & 15) : 0.f;
+    }
+    // s: this lane's plain sum; squares(mean): this lane's sum of squares about a mean.  Returns the row's, in every lane.
+    template <typename F>
+    __device__ __forceinline__ float operator()(float s, F squares, float& mean, const RowPlace<L>& at) {
+        if (L >= 8) {
+            mean = lane_sum<(L >= 8 ? L : 64)>(s) * inv_c;
+            return lane_sum<(L >= 8 ? L : 64)>(squares(mean));
+        }
+        const float m = lane_sum<64>(s) * inv_wave, q = lane_sum<64>(squares(m));
+        float* b = sum.red + sum.turn * (2 * RowSum<L, 2>::PITCH) + at.group * at.waves;
+        sum.turn ^= 1;
+        if ((threadIdx.x & 63) == 0) {
+            b[at.lane >> 6] = m;
+            b[RowSum<L, 2>::PITCH + (at.lane >> 6)] = q;
+        }
+        __syncthreads();
+        const int k = threadIdx.x & 15;
+        const float mk = k < at.waves ? b[k] : 0.f, qk = k < at.waves ? b[RowSum<L, 2>::PITCH + k] : 0.f;
+        mean = lane_sum<16>(n * mk) * inv_c;
+        const float d = mk - mean;
+        return lane_sum<16>(fmaf(n * d, d, qk));
+    }
+};
+
 // one chunk of a row, n elements of it; TINY: the row may be shorter than a chunk
 template <typename T, bool TINY>
 __device__ __forceinline__ u32x4 load_row(const T* p, int n) {
@@ -162,6 +202,15 @@ __device__ __forceinline__ void gate_slopes(float* g, int act) {
     }
 }
 
+// How the gate enters a kernel: constant over the rows that a block goes through (none, per channel, in the backward also per sample: part of
+// the weights), one value per row, or a row of values per row
+enum { GM_CONST = 0, GM_ROW = 1, GM_VECTOR = 2 };
+
+template <typename T, int L, int E>
+int fnet_block_norm_fwd_launch(const FnetBlockNorm& a, hipStream_t st);
+
+// Blocks of a kernel that the GPU holds at once, asked once per kernel, block and LDS size; what the kernel was compiled for if it cannot say
+int fnet_resident_blocks(const void* kernel, int threads, size_t lds, int otherwise);
 int fnet_block_norm_check(const FnetBlockNorm* a);        // the checks that both directions share
 
 #define DISPATCH_ROW(width, ...)                                                   \
@@ -172,3 +221,8 @@ int fnet_block_norm_check(const FnetBlockNorm* a);        // the checks that bot
     else if ((width) <= 2048) { constexpr int L = 1, E = 8; __VA_ARGS__; }         \
     else if ((width) <= 8192) { constexpr int L = 0, E = 8; __VA_ARGS__; }          \
     else { constexpr int L = 0, E = 16; __VA_ARGS__; }
+// the same list, for the instances
+#define FNET_BLOCK_NORM_INSTANCES_OF(X, T) X(T, 8, 8) X(T, 16, 8) X(T, 32, 8) X(T, 64, 8) X(T, 1, 8) X(T, 0, 8) X(T, 0, 16)
+#define FNET_BLOCK_NORM_INSTANCES(T)                              \
+    FNET_BLOCK_NORM_INSTANCES_OF(FNET_BLOCK_NORM_FWD_INSTANCE, T) \
+    FNET_BLOCK_NORM_INSTANCES_OF(FNET_BLOCK_NORM_BWD_INSTANCE, T)

@@ -1,192 +1,44 @@
-// Forward of the norms around a residual block: y = x + a * scale * act(gate) * N(branch), h = N(y), one pass over x, branch and gate.
-#include "fnet_block_norm.h"
+// Norms around a residual block: argument checks, the cut of the rows, the sum of a backward's partial sums and the C entries.  The two large
+// kernels are in fnet_block_norm_fwd.h / fnet_block_norm_bwd.h, compiled once per operand type (fnet_block_norm_{f32,bf16,f16}.hip).
+#include <mutex>
+
+#include "fnet_block_norm_bwd.h"
 
 namespace {
-
-// How the gate enters: constant over the rows (none, per channel: part of the weight in registers), one value per row, or a row of values
-enum { GM_CONST = 0, GM_ROW = 1, GM_VECTOR = 2 };
-
-// One row: load, (mean,) sum of squares about it, the residual sum, and the same for the norm of y, all from registers; y enters the second
-// norm before it is rounded.  The variance is the mean square about the mean, not E[v^2] - mean^2, which loses everything for rows far from
-// zero.  Rows are dealt to blocks in turn; what multiplies a normalised value is loaded once per block.
-template <typename T, int L, int E, int GM, bool LAYER>
-__global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS)) void k_block_norm_fwd(FnetBlockNorm a, RowLaunch rl) {
-    using S = RowShape<T, L, E>;
-    constexpr int V = S::V, K = S::K;
-    __shared__ float red[RowSum<L, 1>::SIZE];
-    RowSum<L, 1> sum(red);
-    const RowPlace<L> at(rl);
-    const int C = a.width;
-    const bool pf = a.param_dtype == FNET_F32, gf = a.gate_dtype == FNET_F32;
-    const float inv_c = 1.f / (float)C;
-    const bool have_branch = a.branch != 0, post = a.post != 0, pre = a.h != 0;
-
-    int col[K], left[K];                             // first element of each of this lane's chunks, and how many of its elements there are
-    bool full = true;
-    float wo[K][V], wy[K][V];                        // residual_scale * scale * post_weight (* act(gate)), pre_weight
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        col[k] = (k * at.lanes + at.lane) * V;
-        left[k] = min(max(C - col[k], 0), V);
-        full = full && left[k] == V;
-        float s[V];
-        load_param_or<T, S::TINY>(a.post_weight, col[k], pf, left[k], 1.f, wo[k]);
-        load_param_or<T, S::TINY>(a.pre_weight, col[k], pf, left[k], 1.f, wy[k]);
-        load_param_or<T, S::TINY>(a.scale, col[k], pf, left[k], 1.f, s);
-#pragma unroll
-        for (int i = 0; i < V; ++i) wo[k][i] *= a.residual_scale * s[i];
-        if (GM == GM_CONST && a.gate) {
-            load_param_or<T, S::TINY>(a.gate, col[k], gf, left[k], 1.f, s);
-            gate_values<V>(s, a.gate_act);
-#pragma unroll
-            for (int i = 0; i < V; ++i) wo[k][i] *= s[i];
-        }
-    }
-    full = __all(full);                              // of this wave: no element of its chunks lies behind the row
-
-    // 1 / deviation of a row (and its mean, taken off)
-    auto normalise = [&](float (&v)[K][V], float& mu) {
-        float s[1];
-        mu = 0.f;
-        if (LAYER) {
-            s[0] = 0.f;
-#pragma unroll
-            for (int k = 0; k < K; ++k)
-#pragma unroll
-                for (int i = 0; i < V; ++i) s[0] += v[k][i];
-            sum(s, at);
-            mu = s[0] * inv_c;
-#pragma unroll
-            for (int k = 0; k < K; ++k)
-#pragma unroll
-                for (int i = 0; i < V; ++i) v[k][i] -= mu;
-            if (!full) {
-#pragma unroll
-                for (int k = 0; k < K; ++k)
-#pragma unroll
-                    for (int i = 0; i < V; ++i) v[k][i] = i < left[k] ? v[k][i] : 0.f;
-            }
-        }
-        s[0] = 0.f;
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int i = 0; i < V; ++i) s[0] = fmaf(v[k][i], v[k][i], s[0]);
-        sum(s, at);
-        return 1.f / sqrtf(s[0] * inv_c + a.eps);
-    };
-
-    // several waves to a row go through the barriers of its sums together: a block's groups take the same number of steps
-    for (long long first = (long long)blockIdx.x * rl.rpb; first < a.rows; first += (long long)gridDim.x * rl.rpb) {
-        const long long row = S::row(first + at.group);
-        const bool here = row < a.rows;
-        if (!S::WAVES && !here) break;
-        float y[K][V], o[K][V];
-        {
-            u32x4 rx[K], ro[K];
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                rx[k] = ro[k] = (u32x4){0u, 0u, 0u, 0u};
-                if (here && left[k] > 0) {
-                    rx[k] = load_row<T, S::TINY>(gptr<const T>(a.x) + row * a.x_stride + col[k], left[k]);
-                    if (have_branch) ro[k] = load_row<T, S::TINY>(gptr<const T>(a.branch) + row * a.branch_stride + col[k], left[k]);
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                unpack16<T>(rx[k], y[k]);
-                unpack16<T>(ro[k], o[k]);
-            }
-        }
-        if (have_branch) {
-            float r = 1.f, mu = 0.f, gt = 1.f;
-            if (GM == GM_ROW && here) gt = gate_value(load_param1<T>(a.gate, row * a.gate_stride, gf), a.gate_act);
-            if (post) {
-                r = normalise(o, mu);
-                if (a.stats && here && at.lane == 0) {
-                    gptr<float>(a.stats)[row] = mu;
-                    gptr<float>(a.stats)[a.rows + row] = r;
-                }
-            }
-            const long long gate_at = GM != GM_VECTOR ? 0 : a.gate_kind == FNET_GATE_ELEMENT ? row * a.gate_stride
-                                      : (long long)((uint32_t)row / (uint32_t)a.tokens) * a.gate_stride;
-            const float rg = GM == GM_ROW ? r * gt : r;
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                float g[V], b[V];
-                if (GM == GM_VECTOR) {
-                    load_param_or<T, S::TINY>(a.gate, gate_at + col[k], gf, here ? left[k] : 0, 0.f, g);
-                    gate_values<V>(g, a.gate_act);
-                }
-                if (a.post_bias) {                   // (v r w + b) = (v r) w + b, with the gate and scale on both
-                    float s[V];
-                    load_param_or<T, S::TINY>(a.post_bias, col[k], pf, left[k], 0.f, b);
-                    load_param_or<T, S::TINY>(a.scale, col[k], pf, left[k], 1.f, s);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) b[i] *= a.residual_scale * s[i];
-                    if (GM == GM_CONST && a.gate) {
-                        load_param_or<T, S::TINY>(a.gate, col[k], gf, left[k], 1.f, s);
-                        gate_values<V>(s, a.gate_act);
-#pragma unroll
-                        for (int i = 0; i < V; ++i) b[i] *= s[i];
-                    }
-                    if (GM == GM_ROW) {
-#pragma unroll
-                        for (int i = 0; i < V; ++i) b[i] *= gt;
-                    }
-#pragma unroll
-                    for (int i = 0; i < V; ++i) o[k][i] = fmaf(o[k][i] * rg, wo[k][i], b[i]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) o[k][i] = o[k][i] * rg * wo[k][i];
-                }
-#pragma unroll
-                for (int i = 0; i < V; ++i) y[k][i] = GM == GM_VECTOR ? fmaf(o[k][i], g[i], y[k][i]) : y[k][i] + o[k][i];
-                if (here && left[k] > 0) store_chunk<T>(gptr<T>(a.y) + row * (long long)C + col[k], left[k], y[k]);
-            }
-        }
-        if (pre) {
-            float mu;
-            const float r = normalise(y, mu);
-            if (a.stats && here && at.lane == 0) {
-                gptr<float>(a.stats)[2 * a.rows + row] = mu;
-                gptr<float>(a.stats)[3 * a.rows + row] = r;
-            }
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                if (a.pre_bias) {
-                    float b[V];
-                    load_param_or<T, S::TINY>(a.pre_bias, col[k], pf, left[k], 0.f, b);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) y[k][i] = fmaf(y[k][i] * r, wy[k][i], b[i]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) y[k][i] = y[k][i] * r * wy[k][i];
-                }
-                if (here && left[k] > 0) store_chunk<T>(gptr<T>(a.h) + row * (long long)C + col[k], left[k], y[k]);
-            }
-        }
-    }
-}
-
-template <typename T, int L, int E>
-void run_fwd(const FnetBlockNorm& a, int gm, hipStream_t st) {
-    const RowLaunch rl = row_launch(L, E, a.width);
-    const long long steps = (a.rows + rl.rpb - 1) / rl.rpb;
-    const long long most = 256 * (2048 / rl.threads);                  // what the chip holds at once
-    const dim3 grid((unsigned)(steps < most ? steps : most)), block(rl.threads);
-    const bool layer = a.kind == FNET_NORM_LAYER;
-#define FNET_FWD(GM, LAYER) hipLaunchKernelGGL((k_block_norm_fwd<T, L, E, GM, LAYER>), grid, block, 0, st, a, rl)
-    if (gm == GM_CONST) { if (layer) FNET_FWD(GM_CONST, true); else FNET_FWD(GM_CONST, false); }
-    else if (gm == GM_ROW) { if (layer) FNET_FWD(GM_ROW, true); else FNET_FWD(GM_ROW, false); }
-    else { if (layer) FNET_FWD(GM_VECTOR, true); else FNET_FWD(GM_VECTOR, false); }
-#undef FNET_FWD
-}
 
 bool type_ok(int d, int operand) { return d == FNET_F32 || d == operand; }
 bool aligned(uint64_t p, int dtype) { return p % (dtype == FNET_F32 ? 4 : 2) == 0; }
 
 }  // namespace
+
+int fnet_resident_blocks(const void* kernel, int threads, size_t lds, int otherwise) {
+    struct Known { const void* kernel; int threads, device; size_t lds; int blocks; };
+    static std::mutex mu;
+    static Known known[1024];
+    static int count = 0;
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return otherwise;
+    std::lock_guard<std::mutex> lock(mu);
+    // open addressing: the few shapes of a program are found at once, and a full table only means asking again
+    size_t h = ((size_t)kernel >> 4) * 31 + threads + lds * 7 + dev;
+    for (int probe = 0; probe < 1024; ++probe, ++h) {
+        Known& k = known[h & 1023];
+        if (k.kernel == kernel && k.threads == threads && k.lds == lds && k.device == dev) return k.blocks;
+        if (k.kernel) continue;
+        int per_cu = 0, cus = 0;
+        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, threads, lds) != hipSuccess || per_cu < 1 ||
+            hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus < 1) {
+            (void)hipGetLastError();
+            return otherwise;
+        }
+        if (count < 1000) {
+            ++count;
+            k = Known{kernel, threads, dev, lds, per_cu * cus};
+        }
+        return per_cu * cus;
+    }
+    return otherwise;
+}
 
 int fnet_block_norm_check(const FnetBlockNorm* a) {
     FNET_CHECK_ARG(a && (a->dtype == FNET_F32 || a->dtype == FNET_BF16 || a->dtype == FNET_F16));
@@ -214,8 +66,168 @@ int fnet_block_norm_fwd(const FnetBlockNorm* host_args, void* stream) {
     if (a.rows == 0) return FNET_OK;
     FNET_CHECK_ARG((a.branch != 0) == (a.y != 0) && (a.y != 0 || a.h != 0) && (a.h != 0 || (a.pre_weight == 0 && a.pre_bias == 0)));
     FNET_CHECK_ARG(aligned(a.y | a.h, a.dtype));
-    const int gm = a.gate_kind == FNET_GATE_TOKEN ? GM_ROW : a.gate_kind == FNET_GATE_ELEMENT || a.gate_kind == FNET_GATE_SAMPLE ? GM_VECTOR : GM_CONST;
-    DISPATCH_T3(a.dtype, DISPATCH_ROW(a.width, { run_fwd<T, L, E>(a, gm, (hipStream_t)stream); }));
+    int out = FNET_OK;
+    DISPATCH_T3(a.dtype, DISPATCH_ROW(a.width, { out = fnet_block_norm_fwd_launch<T, L, E>(a, (hipStream_t)stream); }));
+    return out;
+}
+
+// ---- backward
+namespace {
+
+// out[group][c] = sum over the group's partial rows, in a fixed order: 64 columns by 64 lanes of rows per block, 16 bytes a lane
+struct ColSums {
+    uint64_t src[SUM_COUNT], dst[SUM_COUNT];
+    int groups[SUM_COUNT], slots[SUM_COUNT], f32[SUM_COUNT];
+    int count, width;
+};
+template <typename T>
+__global__ __launch_bounds__(1024) void k_block_norm_cols(ColSums a) {
+    __shared__ float sm[64][65];
+    int e = 0, g = blockIdx.y;
+    while (e + 1 < a.count && g >= a.groups[e]) g -= a.groups[e++];
+    const int cx = (threadIdx.x & 15) * 4, ry = threadIdx.x >> 4, c = blockIdx.x * 64 + cx, C = a.width, slots = a.slots[e], n = C - c;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (n > 0) {
+        const float* p = gptr<const float>(a.src[e]) + (long long)g * slots * C + c;
+        int r = ry;
+        for (; r + 192 < slots; r += 256) {          // four loads under way
+            float v[4][4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) load_chunk<float>(p + (long long)(r + 64 * k) * C, n, v[k]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[i] += v[k][i];
+        }
+        for (; r < slots; r += 64) {
+            float v[4];
+            load_chunk<float>(p + (long long)r * C, n, v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] += v[i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sm[ry][cx + i] = s[i];
+    __syncthreads();
+    const int col = threadIdx.x >> 4, l = threadIdx.x & 15, o = blockIdx.x * 64 + col;
+    const float t = lane_sum<16>((sm[l][col] + sm[l + 16][col]) + (sm[l + 32][col] + sm[l + 48][col]));
+    if (l == 0 && o < C) {
+        if (a.f32[e]) gptr<float>(a.dst[e])[(long long)g * C + o] = t;
+        else gptr<T>(a.dst[e])[(long long)g * C + o] = f_to_elem<T>(t);
+    }
+}
+
+struct BwdShape {
+    BwdPlan plan;
+    RowLaunch rl;
+    int blocks, gm;
+    bool bias;
+    long long bytes;             // of partial sums
+};
+constexpr int kMinSteps = 4;     // steps of a block's rows at least, where there are that many: a block's partial sums cost as much as a row
+
+// How the rows are cut: blocks that fill the chip once, each with a run of rows; with a gate per sample a run ends with its sample, so that
+// what the gate multiplies is constant over it.
+// most: blocks that the GPU holds at once, as far as that is known (the workspace is of the most that there may be).
+void bwd_shape(const FnetBlockNorm& a, int L, int E, int most, BwdShape* out) {
+    BwdPlan p{};
+    out->rl = row_launch(L, E, a.width);
+    const int rpb = out->rl.rpb;
+    const bool by_sample = a.gate_kind == FNET_GATE_SAMPLE;
+    p.samples = by_sample ? (int)(a.rows / a.tokens) : 1;
+    p.sample_rows = by_sample ? a.tokens : a.rows;
+    out->gm = a.gate_kind == FNET_GATE_TOKEN ? GM_ROW : a.gate_kind == FNET_GATE_ELEMENT ? GM_VECTOR : GM_CONST;
+    out->bias = a.post_bias || a.dpost_bias || a.dpre_bias;
+    const int per_cu = 1024 / out->rl.threads, chip = 256 * (per_cu > 1 ? per_cu : 1);     // 16 waves of 128 registers on a CU
+    const long long target = most > 0 && most < chip ? most : chip;
+    const long long steps = (p.sample_rows + rpb - 1) / rpb;
+    long long parts = target / p.samples;
+    if (parts > steps / kMinSteps) parts = steps / kMinSteps;
+    if (parts < 1) parts = 1;
+    p.part_rows = ((steps + parts - 1) / parts) * rpb;
+    p.parts = (int)((p.sample_rows + p.part_rows - 1) / p.part_rows);
+    const long long segments = (long long)p.samples * p.parts;
+    out->blocks = (int)(segments < target ? segments : target);
+    out->bytes = 0;
+    const uint64_t want[SUM_COUNT] = {a.dpre_weight, a.dpre_bias, a.dpost_weight, a.dpost_bias, a.dscale, out->gm == GM_CONST ? a.dgate : 0};
+    for (int s = 0; s < SUM_COUNT; ++s) {
+        if (!want[s]) continue;
+        const long long rows = s >= SUM_POST_W ? segments : out->blocks;
+        if (s == SUM_GATE && by_sample ? p.parts == 1 : rows == 1) {
+            p.direct |= 1 << s;
+            p.dst[s] = want[s];
+        } else {
+            p.dst[s] = a.workspace + out->bytes;
+            out->bytes += (rows * a.width * 4 + 15) / 16 * 16;
+        }
+    }
+    out->plan = p;
+}
+
+int bwd_check(const FnetBlockNorm* a) {
+    const int rc = fnet_block_norm_check(a);
+    if (rc != FNET_OK) return rc;
+    FNET_CHECK_ARG(a->branch != 0 || (!a->dbranch && !a->dgate && !a->dscale));
+    FNET_CHECK_ARG(a->post || (!a->dpost_weight && !a->dpost_bias));
+    FNET_CHECK_ARG(a->gate_kind != FNET_GATE_NONE || !a->dgate);
+    const auto ok = [](uint64_t p, int dtype) { return p % (dtype == FNET_F32 ? 4 : 2) == 0; };
+    FNET_CHECK_ARG(ok(a->dy | a->dh | a->dx | a->dbranch, a->dtype) && ok(a->dgate, a->gate_dtype));
+    FNET_CHECK_ARG(ok(a->dscale | a->dpost_weight | a->dpost_bias | a->dpre_weight | a->dpre_bias, a->param_dtype));
+    return FNET_OK;
+}
+
+template <typename T, int L, int E>
+int run_bwd(const FnetBlockNorm& a, hipStream_t st) {
+    BwdShape s;
+    bwd_shape(a, L, E, 0, &s);
+    FNET_CHECK_ARG(s.bytes == 0 || (a.workspace != 0 && a.workspace % 16 == 0 && a.workspace_bytes >= s.bytes));
+    const int most = fnet_block_norm_bwd_resident<T, L, E>(s.rl, s.gm, s.bias, a.kind == FNET_NORM_LAYER);
+    if (most < s.blocks) bwd_shape(a, L, E, most, &s);
+    const int rc = fnet_block_norm_bwd_launch<T, L, E>(a, s.plan, s.rl, s.blocks, s.gm, s.bias, st);
+    if (rc != FNET_OK) return rc;
+    FNET_LAUNCH_CHECK();
+    if (s.bytes == 0) return FNET_OK;
+    ColSums c{};
+    c.width = a.width;
+    const uint64_t out[SUM_COUNT] = {a.dpre_weight, a.dpre_bias, a.dpost_weight, a.dpost_bias, a.dscale, a.dgate};
+    int groups = 0;
+    for (int i = 0; i < SUM_COUNT; ++i) {
+        if (!s.plan.dst[i] || (s.plan.direct >> i) & 1) continue;
+        const bool by_sample = i == SUM_GATE && a.gate_kind == FNET_GATE_SAMPLE;
+        c.src[c.count] = s.plan.dst[i];
+        c.dst[c.count] = out[i];
+        c.groups[c.count] = by_sample ? s.plan.samples : 1;
+        c.slots[c.count] = by_sample ? s.plan.parts : i >= SUM_POST_W ? s.plan.samples * s.plan.parts : s.blocks;
+        c.f32[c.count] = (i == SUM_GATE ? a.gate_dtype : a.param_dtype) == FNET_F32;
+        groups += c.groups[c.count++];
+    }
+    hipLaunchKernelGGL(k_block_norm_cols<T>, dim3((a.width + 63) / 64, groups), dim3(1024), 0, st, c);
     FNET_LAUNCH_CHECK();
     return FNET_OK;
+}
+
+}  // namespace
+
+int fnet_block_norm_workspace(const FnetBlockNorm* host_args, int64_t* bytes) {
+    FNET_CHECK_ARG(bytes);
+    const int rc = bwd_check(host_args);
+    if (rc != FNET_OK) return rc;
+    *bytes = 0;
+    if (host_args->rows == 0) return FNET_OK;
+    BwdShape s;
+    DISPATCH_ROW(host_args->width, { bwd_shape(*host_args, L, E, 0, &s); });
+    *bytes = s.bytes;
+    return FNET_OK;
+}
+
+int fnet_block_norm_bwd(const FnetBlockNorm* host_args, void* stream) {
+    const int rc = bwd_check(host_args);
+    if (rc != FNET_OK) return rc;
+    const FnetBlockNorm& a = *host_args;
+    if (a.rows == 0) return FNET_OK;
+    FNET_CHECK_ARG((!a.post && !a.dh) || a.stats != 0);
+    FNET_CHECK_ARG(a.dh != 0 || (!a.dpre_weight && !a.dpre_bias));
+    int out = FNET_OK;
+    DISPATCH_T3(a.dtype, DISPATCH_ROW(a.width, { out = run_bwd<T, L, E>(a, (hipStream_t)stream); }));
+    return out;
 }

@@ -1,4 +1,4 @@
-// The backward kernel of the norms around a residual block, for one operand type; fnet_block_norm_bwd_{f32,bf16,f16}.hip instantiate it.
+// The backward kernel of the norms around a residual block, for one operand type; fnet_block_norm_{f32,bf16,f16}.hip instantiate it.
 #pragma once
 #include "fnet_block_norm.h"
 
@@ -14,18 +14,20 @@ struct BwdPlan {
     long long sample_rows, part_rows;
 };
 
-// How the gate enters: constant over a segment's rows (none, per channel, per sample), one value per row, or a row of values per row
-enum { GM_CONST = 0, GM_ROW = 1, GM_VECTOR = 2 };
-
 // Waves per SIMD that the kernel is compiled for: 4 leave 128 registers to each; two more sums or a gate in registers do not fit those, and
 // 3 waves without spilling are faster than 4 with it.  Blocks of more than 8 waves leave no choice.
 constexpr int bwd_waves(int L, int gm, bool bias) { return (bias || gm == GM_VECTOR) && L != 0 ? 3 : 4; }
 
-// one instance: launches the kernel (bias: sums for biases too)
-template <typename T, int L, int E>
-void fnet_block_norm_bwd_launch(const FnetBlockNorm& a, const BwdPlan& plan, const RowLaunch& rl, int blocks, int gm, bool bias, hipStream_t st);
+// arrays of weights that the kernel keeps in the LDS; rows of more than 8192 elements leave no room for the third
+constexpr int bwd_lds_arrays(int E, bool bias) { return bias && E == 8 ? 3 : 2; }
 
-#ifdef FNET_BLOCK_NORM_BWD_KERNEL
+// one instance: launches the kernel (bias: sums for biases too); how many of its blocks the GPU holds
+template <typename T, int L, int E>
+int fnet_block_norm_bwd_resident(const RowLaunch& rl, int gm, bool bias, bool layer);
+template <typename T, int L, int E>
+int fnet_block_norm_bwd_launch(const FnetBlockNorm& a, const BwdPlan& plan, const RowLaunch& rl, int blocks, int gm, bool bias, hipStream_t st);
+
+#ifdef FNET_BLOCK_NORM_KERNELS
 namespace {
 
 // The sums of a block's row groups into row `row` of `dst`: through LDS, group by group in order.
@@ -70,12 +72,13 @@ __device__ __forceinline__ void leave_sum(const float (&acc)[RowShape<T, L, E>::
 //   dpost_weight = residual_scale * scale * sum f d z,  dpost_bias = residual_scale * scale * sum f d,
 //   dscale = residual_scale * (post_weight * sum f d z + post_bias * sum f d)
 // so two sums over rows (one without biases) give every gradient on the branch's side, and where f is constant over the rows it enters only
-// when they are left: f is part of W and B in registers, and dgate of a channel or sample comes from the same two sums.
+// when they are left: f is part of W and B, and dgate of a channel or sample comes from the same two sums.
 // A row's arithmetic is 18 to 40 operations an element, which keeps it below the time of the 10 to 14 bytes it moves (bf16).
 template <typename T, int L, int E, int GM, bool LAYER, bool BIAS>
 __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, BIAS)) void k_block_norm_bwd(FnetBlockNorm a, BwdPlan plan, RowLaunch rl) {
     using S = RowShape<T, L, E>;
     constexpr int V = S::V, K = S::K;
+    constexpr bool WY_LDS = bwd_lds_arrays(E, BIAS) == (BIAS ? 3 : 2);
     __shared__ float red[RowSum<L, 3>::SIZE];
     __shared__ float sm[L ? 256 * E : 1];            // several row groups: 256 lanes
     RowSum<L, 3> sum(red);
@@ -90,38 +93,70 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
 
     int col[K], left[K];
     bool full = true;
-    float wy[K][V], wo[K][V], bo[BIAS ? K : 1][V];    // pre_weight; W and B above (with f, where that is constant)
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         col[k] = (k * at.lanes + at.lane) * V;
         left[k] = min(max(C - col[k], 0), V);
         full = full && left[k] == V;
-        load_param_or<T, S::TINY>(a.pre_weight, col[k], pf, left[k], 1.f, wy[k]);
     }
     full = __all(full);
+
+    // pre_weight, W and B (above; with f, where that is constant) lie in the LDS, for all rows of the block: in registers they would cost
+    // a wave in flight.  Four of a chunk's values to a plane, so that the lanes' 16-byte reads lie side by side.
+    extern __shared__ float weights[];
+    const int plane = at.lanes * K * 4, pitch = plane * (V / 4);
+    float wy_reg[WY_LDS ? 1 : K][V];
+    auto put = [&](int which, int k, const float* v) {
+        if (at.group == 0) {
+#pragma unroll
+            for (int p = 0; p < V / 4; ++p)
+                *reinterpret_cast<float4*>(weights + which * pitch + p * plane + (k * at.lanes + at.lane) * 4) = make_float4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
+        }
+    };
+    auto get = [&](int which, int k, float* v) {
+#pragma unroll
+        for (int p = 0; p < V / 4; ++p) {
+            const float4 w = *reinterpret_cast<const float4*>(weights + which * pitch + p * plane + (k * at.lanes + at.lane) * 4);
+            v[4 * p] = w.x; v[4 * p + 1] = w.y; v[4 * p + 2] = w.z; v[4 * p + 3] = w.w;
+        }
+    };
+    enum { W_O = 0, W_B = 1, W_Y = BIAS ? 2 : 1 };
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        float w[V];
+        load_param_or<T, S::TINY>(a.pre_weight, col[k], pf, left[k], 1.f, w);
+        if (WY_LDS) put(W_Y, k, w);
+        else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) wy_reg[WY_LDS ? 0 : k][i] = w[i];
+        }
+    }
     auto load_branch_side = [&](long long gate_at) {
+        __syncthreads();                             // the segment before has been read
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            float s[V];
+            float s[V], w[V];
             load_param_or<T, S::TINY>(a.scale, col[k], pf, left[k], 1.f, s);
 #pragma unroll
             for (int i = 0; i < V; ++i) s[i] *= a.residual_scale;
             if (GM == GM_CONST && a.gate) {
-                float g[V];
-                load_param_or<T, S::TINY>(a.gate, gate_at + col[k], gf, left[k], 1.f, g);
-                gate_values<V>(g, a.gate_act);
+                load_param_or<T, S::TINY>(a.gate, gate_at + col[k], gf, left[k], 1.f, w);
+                gate_values<V>(w, a.gate_act);
 #pragma unroll
-                for (int i = 0; i < V; ++i) s[i] *= g[i];
+                for (int i = 0; i < V; ++i) s[i] *= w[i];
             }
-            load_param_or<T, S::TINY>(a.post_weight, col[k], pf, left[k], 1.f, wo[k]);
+            load_param_or<T, S::TINY>(a.post_weight, col[k], pf, left[k], 1.f, w);
 #pragma unroll
-            for (int i = 0; i < V; ++i) wo[k][i] *= s[i];
+            for (int i = 0; i < V; ++i) w[i] *= s[i];
+            put(W_O, k, w);
             if (BIAS) {
-                load_param_or<T, S::TINY>(a.post_bias, col[k], pf, left[k], 0.f, bo[BIAS ? k : 0]);
+                load_param_or<T, S::TINY>(a.post_bias, col[k], pf, left[k], 0.f, w);
 #pragma unroll
-                for (int i = 0; i < V; ++i) bo[BIAS ? k : 0][i] *= s[i];
+                for (int i = 0; i < V; ++i) w[i] *= s[i];
+                put(W_B, k, w);
             }
         }
+        __syncthreads();
     };
 
     float ay[K][V], ay0[BIAS ? K : 1][V], ao[K][V], ao0[BIAS ? K : 1][V];       // sums of dh y_hat, dh, f d z, f d
@@ -169,37 +204,44 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
         const long long end = min(first + plan.part_rows, (sample + 1) * plan.sample_rows);
         const long long sample_gate = a.gate_kind == FNET_GATE_SAMPLE ? (long long)sample * a.gate_stride : 0;
         load_branch_side(sample_gate);
+        struct Row {
+            u32x4 x[K], o[K], d[K], t[K];            // x, branch, dy, dh as loaded
+            float mu_o, r_o, mu_y, r_y, gate;
+        };
+        auto load = [&](long long row, bool here, Row& r) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                r.x[k] = r.o[k] = r.d[k] = r.t[k] = (u32x4){0u, 0u, 0u, 0u};
+                if (here && left[k] > 0) {
+                    if (need_branch) r.o[k] = load_row<T, S::TINY>(gptr<const T>(a.branch) + row * a.branch_stride + col[k], left[k]);
+                    if (pre) {
+                        r.x[k] = load_row<T, S::TINY>(gptr<const T>(a.x) + row * a.x_stride + col[k], left[k]);
+                        r.t[k] = load_row<T, S::TINY>(gptr<const T>(a.dh) + row * a.dh_stride + col[k], left[k]);
+                    }
+                    if (a.dy) r.d[k] = load_row<T, S::TINY>(gptr<const T>(a.dy) + row * a.dy_stride + col[k], left[k]);
+                }
+            }
+            r.mu_o = r.mu_y = r.gate = 0.f;
+            r.r_o = r.r_y = 1.f;
+            if (here) {
+                if (post) { r.mu_o = gptr<const float>(a.stats)[row]; r.r_o = gptr<const float>(a.stats)[a.rows + row]; }
+                if (pre) { r.mu_y = gptr<const float>(a.stats)[2 * a.rows + row]; r.r_y = gptr<const float>(a.stats)[3 * a.rows + row]; }
+                if (GM == GM_ROW) r.gate = load_param1<T>(a.gate, row * a.gate_stride, gf);
+            }
+        };
         // several waves to a row go through the barriers of its sums together: a block's groups take the same number of steps
         for (long long step = first; step < end; step += groups) {
             const long long row = S::row(step + at.group);
             const bool here = row < end;
             if (!S::WAVES && !here) break;
-            u32x4 rx[K], ro[K], rd[K], rt[K];
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                rx[k] = ro[k] = rd[k] = rt[k] = (u32x4){0u, 0u, 0u, 0u};
-                if (here && left[k] > 0) {
-                    if (pre) {
-                        rt[k] = load_row<T, S::TINY>(gptr<const T>(a.dh) + row * a.dh_stride + col[k], left[k]);
-                        rx[k] = load_row<T, S::TINY>(gptr<const T>(a.x) + row * a.x_stride + col[k], left[k]);
-                    }
-                    if (need_branch) ro[k] = load_row<T, S::TINY>(gptr<const T>(a.branch) + row * a.branch_stride + col[k], left[k]);
-                    if (a.dy) rd[k] = load_row<T, S::TINY>(gptr<const T>(a.dy) + row * a.dy_stride + col[k], left[k]);
-                }
-            }
-            float mu_o = 0.f, r_o = 1.f, mu_y = 0.f, r_y = 1.f, gt = 0.f, ft = 1.f;
-            if (here) {
-                if (post) { mu_o = gptr<const float>(a.stats)[row]; r_o = gptr<const float>(a.stats)[a.rows + row]; }
-                if (pre) { mu_y = gptr<const float>(a.stats)[2 * a.rows + row]; r_y = gptr<const float>(a.stats)[3 * a.rows + row]; }
-                if (GM == GM_ROW) {
-                    gt = load_param1<T>(a.gate, row * a.gate_stride, gf);
-                    ft = gate_value(gt, a.gate_act);
-                }
-            }
+            Row now;
+            load(row, here, now);
+            const float mu_o = now.mu_o, r_o = now.r_o, mu_y = now.mu_y, r_y = now.r_y, gt = now.gate;
+            const float ft = GM == GM_ROW ? gate_value(gt, a.gate_act) : 1.f;
             float z[K][V], d[K][V], f[GM == GM_VECTOR ? K : 1][V];
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                unpack16<T>(ro[k], z[k]);
+                unpack16<T>(now.o[k], z[k]);
                 if (GM == GM_VECTOR) {
                     float(&fk)[V] = f[GM == GM_VECTOR ? k : 0];
                     load_param_or<T, S::TINY>(a.gate, row * a.gate_stride + col[k], gf, here ? left[k] : 0, 0.f, fk);
@@ -212,25 +254,33 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
             }
             if (!pre) {
 #pragma unroll
-                for (int k = 0; k < K; ++k) unpack16<T>(rd[k], d[k]);
+                for (int k = 0; k < K; ++k) unpack16<T>(now.d[k], d[k]);
             } else {
                 float y[K][V], t[K][V], s2[2] = {0.f, 0.f};
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
-                    unpack16<T>(rx[k], y[k]);
-                    unpack16<T>(rt[k], t[k]);
+                    unpack16<T>(now.x[k], y[k]);
+                    unpack16<T>(now.t[k], t[k]);
+                    float wo[V], bo[V], wy[V];
+                    get(W_O, k, wo);
+                    if (BIAS) get(W_B, k, bo);
+                    if (WY_LDS) get(W_Y, k, wy);
+                    else {
+#pragma unroll
+                        for (int i = 0; i < V; ++i) wy[i] = wy_reg[WY_LDS ? 0 : k][i];
+                    }
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
                         if (GM == GM_CONST) {
-                            y[k][i] = fmaf(wo[k][i], z[k][i], BIAS ? y[k][i] + bo[BIAS ? k : 0][i] : y[k][i]);
+                            y[k][i] = fmaf(wo[i], z[k][i], BIAS ? y[k][i] + bo[i] : y[k][i]);
                         } else {
-                            const float u = BIAS ? fmaf(wo[k][i], z[k][i], bo[BIAS ? k : 0][i]) : wo[k][i] * z[k][i];
+                            const float u = BIAS ? fmaf(wo[i], z[k][i], bo[i]) : wo[i] * z[k][i];
                             y[k][i] = fmaf(GM == GM_ROW ? ft : f[GM == GM_VECTOR ? k : 0][i], u, y[k][i]);
                         }
                         y[k][i] = LAYER ? (y[k][i] - mu_y) * r_y : y[k][i] * r_y;
                         ay[k][i] = fmaf(t[k][i], y[k][i], ay[k][i]);
                         if (BIAS) ay0[BIAS ? k : 0][i] += t[k][i];
-                        t[k][i] *= wy[k][i];
+                        t[k][i] *= wy[i];
                         if (LAYER) s2[0] += t[k][i];
                         s2[1] = fmaf(t[k][i], y[k][i], s2[1]);
                     }
@@ -245,7 +295,7 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
                 const float m0 = LAYER ? s2[0] * inv_c : 0.f, m1 = s2[1] * inv_c;
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
-                    unpack16<T>(rd[k], d[k]);        // held as loaded until here: registers are what limits the waves in flight
+                    unpack16<T>(now.d[k], d[k]);        // held as loaded until here: registers are what limits the waves in flight
 #pragma unroll
                     for (int i = 0; i < V; ++i) d[k][i] = fmaf(r_y, fmaf(-m1, y[k][i], LAYER ? t[k][i] - m0 : t[k][i]), d[k][i]);
                 }
@@ -265,6 +315,9 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
                 float s3[3] = {0.f, 0.f, 0.f};       // sums of q, q z and, per row, d B; q = d W, with the row's f put in after the sums
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
+                    float wo[V], bo[V];
+                    get(W_O, k, wo);
+                    if (BIAS) get(W_B, k, bo);
                     if (GM == GM_VECTOR) {
                         float(&fk)[V] = f[GM == GM_VECTOR ? k : 0];
                         if (a.dgate) {
@@ -272,7 +325,7 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
                             load_param_or<T, S::TINY>(a.gate, row * a.gate_stride + col[k], gf, here ? left[k] : 0, 0.f, g);
                             gate_slopes<V>(g, a.gate_act);
 #pragma unroll
-                            for (int i = 0; i < V; ++i) g[i] *= d[k][i] * (BIAS ? fmaf(wo[k][i], z[k][i], bo[BIAS ? k : 0][i]) : wo[k][i] * z[k][i]);
+                            for (int i = 0; i < V; ++i) g[i] *= d[k][i] * (BIAS ? fmaf(wo[i], z[k][i], bo[i]) : wo[i] * z[k][i]);
                             if (here && left[k] > 0) store_param<T>(a.dgate, row * (long long)C + col[k], gf, left[k], g);
                         }
 #pragma unroll
@@ -283,8 +336,8 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
                         const float fd = GM == GM_ROW ? ft * d[k][i] : d[k][i];
                         ao[k][i] = fmaf(fd, z[k][i], ao[k][i]);
                         if (BIAS) ao0[BIAS ? k : 0][i] += fd;
-                        if (GM == GM_ROW && BIAS) s3[2] = fmaf(d[k][i], bo[BIAS ? k : 0][i], s3[2]);
-                        d[k][i] *= wo[k][i];
+                        if (GM == GM_ROW && BIAS) s3[2] = fmaf(d[k][i], bo[i], s3[2]);
+                        d[k][i] *= wo[i];
                         if (LAYER) s3[0] += d[k][i];
                         s3[1] = fmaf(d[k][i], z[k][i], s3[1]);
                     }
@@ -329,23 +382,35 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
 }  // namespace
 
 template <typename T, int L, int E>
-void fnet_block_norm_bwd_launch(const FnetBlockNorm& a, const BwdPlan& plan, const RowLaunch& rl, int blocks, int gm, bool bias, hipStream_t st) {
-    const dim3 grid(blocks), block(rl.threads);
-    const bool layer = a.kind == FNET_NORM_LAYER;
-#define FNET_BWD3(GM, LAYER, BIAS) hipLaunchKernelGGL((k_block_norm_bwd<T, L, E, GM, LAYER, BIAS>), grid, block, 0, st, a, plan, rl)
-#define FNET_BWD(GM)                                                                    \
-    if (layer) { if (bias) FNET_BWD3(GM, true, true); else FNET_BWD3(GM, true, false); } \
-    else { if (bias) FNET_BWD3(GM, false, true); else FNET_BWD3(GM, false, false); }
-    if (gm == GM_CONST) { FNET_BWD(GM_CONST) }
-    else if (gm == GM_ROW) { FNET_BWD(GM_ROW) }
-    else { FNET_BWD(GM_VECTOR) }
+const void* bwd_kernel(int gm, bool layer, bool bias) {
+#define FNET_BWD(GM)                                                                                                                 \
+    (layer ? (bias ? (const void*)k_block_norm_bwd<T, L, E, GM, true, true> : (const void*)k_block_norm_bwd<T, L, E, GM, true, false>) \
+           : (bias ? (const void*)k_block_norm_bwd<T, L, E, GM, false, true> : (const void*)k_block_norm_bwd<T, L, E, GM, false, false>))
+    return gm == GM_CONST ? FNET_BWD(GM_CONST) : gm == GM_ROW ? FNET_BWD(GM_ROW) : FNET_BWD(GM_VECTOR);
 #undef FNET_BWD
-#undef FNET_BWD3
+}
+inline int bwd_lds_bytes(int L, int E, const RowLaunch& rl, bool bias) { return bwd_lds_arrays(E, bias) * (L >= 8 ? L : 64 * rl.waves) * E * 4; }
+
+template <typename T, int L, int E>
+int fnet_block_norm_bwd_resident(const RowLaunch& rl, int gm, bool bias, bool layer) {
+    return fnet_resident_blocks(bwd_kernel<T, L, E>(gm, layer, bias), rl.threads, bwd_lds_bytes(L, E, rl, bias), 256 * 1024 / rl.threads);
+}
+template <typename T, int L, int E>
+int fnet_block_norm_bwd_launch(const FnetBlockNorm& a, const BwdPlan& plan, const RowLaunch& rl, int blocks, int gm, bool bias, hipStream_t st) {
+    const void* kernel = bwd_kernel<T, L, E>(gm, a.kind == FNET_NORM_LAYER, bias);
+    const int lds = bwd_lds_bytes(L, E, rl, bias);
+    hipError_t e = hipSuccess;
+    if (lds > 32768)                                 // with the kernel's static LDS this may pass what is granted without asking
+        e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    FnetBlockNorm arg = a;
+    BwdPlan p = plan;
+    RowLaunch r = rl;
+    void* args[] = {&arg, &p, &r};
+    if (e == hipSuccess) e = hipLaunchKernel(kernel, dim3(blocks), dim3(rl.threads), args, lds, st);
+    if (e != hipSuccess) { g_fnet_last_hip_error = (int)e; return FNET_E_HIP; }
+    return FNET_OK;
 }
 #define FNET_BLOCK_NORM_BWD_INSTANCE(T, L, E)                                                                                          \
-    template void fnet_block_norm_bwd_launch<T, L, E>(const FnetBlockNorm&, const BwdPlan&, const RowLaunch&, int, int, bool, hipStream_t);
-#define FNET_BLOCK_NORM_BWD_INSTANCES(T)                                                              \
-    FNET_BLOCK_NORM_BWD_INSTANCE(T, 8, 8) FNET_BLOCK_NORM_BWD_INSTANCE(T, 16, 8)                       \
-    FNET_BLOCK_NORM_BWD_INSTANCE(T, 32, 8) FNET_BLOCK_NORM_BWD_INSTANCE(T, 64, 8)                      \
-    FNET_BLOCK_NORM_BWD_INSTANCE(T, 1, 8) FNET_BLOCK_NORM_BWD_INSTANCE(T, 0, 8) FNET_BLOCK_NORM_BWD_INSTANCE(T, 0, 16)
+    template int fnet_block_norm_bwd_resident<T, L, E>(const RowLaunch&, int, bool, bool);                                            \
+    template int fnet_block_norm_bwd_launch<T, L, E>(const FnetBlockNorm&, const BwdPlan&, const RowLaunch&, int, int, bool, hipStream_t);
 #endif
