@@ -123,25 +123,35 @@ struct RowMoments {
     }
 };
 
-// one chunk of a row, n elements of it; TINY: the row may be shorter than a chunk
+// one chunk of a row, n elements of it (n > 0); TINY: the row may be shorter than a chunk.  align_row completes it.
 template <typename T, bool TINY>
 __device__ __forceinline__ u32x4 load_row(const T* p, int n) {
-    return TINY ? load_raw<T>(p, n) : load_row_raw<T>(p, n);
+    return TINY ? load_raw<T>(p, n) : load_row_end<T>(p, n);
+}
+template <typename T, bool TINY>
+__device__ __forceinline__ void align_row(u32x4& w, int n) {
+    if (!TINY && n > 0) shift_row<T>(w, n);
 }
 // one chunk of a parameter (or gate) that is fp32 or of the operands' type
 template <typename T, bool TINY>
 __device__ __forceinline__ void load_param(uint64_t p, long long at, bool f32, int n, float* v) {
     if (f32 && VecOf<T>::V == 8) {
         const float* q = gptr<const float>(p) + at;
-        const u32x4 lo = load_row<float, TINY>(q, min(n, 4));
-        const u32x4 hi = n > 4 ? load_row<float, TINY>(q + 4, n - 4) : (u32x4){0u, 0u, 0u, 0u};
+        u32x4 lo = load_row<float, TINY>(q, min(n, 4)), hi = {0u, 0u, 0u, 0u};
+        if (n > 4) hi = load_row<float, TINY>(q + 4, n - 4);
+        if (n < 8) {
+            align_row<float, TINY>(lo, min(n, 4));
+            align_row<float, TINY>(hi, n - 4);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             v[i] = __uint_as_float(lo[i]);
             v[VecOf<T>::V - 4 + i] = __uint_as_float(hi[i]);
         }
     } else {
-        unpack16<T>(load_row<T, TINY>(gptr<const T>(p) + at, n), v);
+        u32x4 w = load_row<T, TINY>(gptr<const T>(p) + at, n);
+        if (n < VecOf<T>::V) align_row<T, TINY>(w, n);
+        unpack16<T>(w, v);
     }
 }
 // the same of a parameter that may be absent (then `absent`), and of a chunk that may lie behind the row (then zero)

@@ -228,6 +228,15 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
                 if (pre) { r.mu_y = gptr<const float>(a.stats)[2 * a.rows + row]; r.r_y = gptr<const float>(a.stats)[3 * a.rows + row]; }
                 if (GM == GM_ROW) r.gate = load_param1<T>(a.gate, row * a.gate_stride, gf);
             }
+            if (!full) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    align_row<T, S::TINY>(r.o[k], left[k]);
+                    align_row<T, S::TINY>(r.x[k], left[k]);
+                    align_row<T, S::TINY>(r.t[k], left[k]);
+                    align_row<T, S::TINY>(r.d[k], left[k]);
+                }
+            }
         };
         // several waves to a row go through the barriers of its sums together: a block's groups take the same number of steps
         for (long long step = first; step < end; step += groups) {

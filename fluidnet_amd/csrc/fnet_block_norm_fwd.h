@@ -114,6 +114,13 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS)) void k_block_norm
                     if (have_branch) ro[k] = load_row<T, S::TINY>(gptr<const T>(a.branch) + row * a.branch_stride + col[k], left[k]);
                 }
             }
+            if (!full) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    align_row<T, S::TINY>(rx[k], left[k]);
+                    align_row<T, S::TINY>(ro[k], left[k]);
+                }
+            }
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 unpack16<T>(rx[k], y[k]);

@@ -102,29 +102,30 @@ __device__ __forceinline__ void store_chunk(T* p, int n, const float* v) {
     }
 }
 
-// The same for a chunk that ends a row of at least V elements: the 16 bytes that end where the row ends, shifted down to the chunk's own
-// place (one load and a dozen operations instead of a load per element).
+// The same for a chunk that ends a row of at least V elements: the 16 bytes that end where the row ends, and shift_row to move them down to
+// the chunk's own place (one load and a dozen operations instead of a load per element).  Two steps, because the second has to wait for the
+// first: a row's loads are all issued before any of them is shifted.
 template <typename T>
-__device__ __forceinline__ u32x4 load_row_raw(const T* p, int n) {
+__device__ __forceinline__ u32x4 load_row_end(const T* p, int n) {
+    return *reinterpret_cast<const typename VecOf<T>::vec*>(p - (VecOf<T>::V - n));
+}
+template <typename T>
+__device__ __forceinline__ void shift_row(u32x4& w, int n) {
     constexpr int V = VecOf<T>::V;
     const int s = V - n;                             // 0 for a whole chunk
-    u32x4 w = *reinterpret_cast<const typename VecOf<T>::vec*>(p - s);
-    if (s) {
-        if (V == 8) {
-            const u32x4 h = {__builtin_amdgcn_alignbit(w[1], w[0], 16), __builtin_amdgcn_alignbit(w[2], w[1], 16),
-                             __builtin_amdgcn_alignbit(w[3], w[2], 16), w[3] >> 16};
+    if (V == 8) {
+        const u32x4 h = {__builtin_amdgcn_alignbit(w[1], w[0], 16), __builtin_amdgcn_alignbit(w[2], w[1], 16),
+                         __builtin_amdgcn_alignbit(w[3], w[2], 16), w[3] >> 16};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = (s & 1) ? h[k] : w[k];
-        }
-        const int d = V == 8 ? s >> 1 : s;           // in words
-        const u32x4 one = {w[1], w[2], w[3], 0u};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = (d & 1) ? one[k] : w[k];
-        const u32x4 two = {w[2], w[3], 0u, 0u};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = (d & 2) ? two[k] : w[k];
+        for (int k = 0; k < 4; ++k) w[k] = (s & 1) ? h[k] : w[k];
     }
-    return w;
+    const int d = V == 8 ? s >> 1 : s;               // in words
+    const u32x4 one = {w[1], w[2], w[3], 0u};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = (d & 1) ? one[k] : w[k];
+    const u32x4 two = {w[2], w[3], 0u, 0u};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = (d & 2) ? two[k] : w[k];
 }
 
 // Sum over groups of L consecutive lanes (L = 8 .. 64, a power of two), the result in every lane of the group.  Inside 16 lanes by DPP:
