@@ -30,42 +30,6 @@ int fnet_block_norm_bwd_launch(const FnetBlockNorm& a, const BwdPlan& plan, cons
 #ifdef FNET_BLOCK_NORM_KERNELS
 namespace {
 
-// The sums of a block's row groups into row `row` of `dst`: through LDS, group by group in order.
-template <typename T, int L, int E>
-__device__ __forceinline__ void leave_sum(const float (&acc)[RowShape<T, L, E>::K][RowShape<T, L, E>::V], uint64_t dst, long long row, int C,
-                                          bool direct, bool f32, float* sm, const RowPlace<L>& at, int groups) {
-    constexpr int V = RowShape<T, L, E>::V, K = RowShape<T, L, E>::K;
-    if (groups == 1) {
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int c = (k * at.lanes + at.lane) * V, n = min(C - c, V);
-            if (n <= 0) continue;
-            if (direct) {
-                store_param<T>(dst, row * C + c, f32, n, acc[k]);
-            } else {
-                float* q = gptr<float>(dst) + row * C + c;
-#pragma unroll
-                for (int i = 0; i < V; i += 4)
-                    if (n > i) store_chunk<float>(q + i, n - i, &acc[k][i]);
-            }
-        }
-        return;
-    }
-    const int pitch = at.lanes * E;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < V; ++i) sm[at.group * pitch + (k * at.lanes + at.lane) * V + i] = acc[k][i];
-    __syncthreads();
-    for (int c = threadIdx.x; c < C; c += blockDim.x) {
-        float s = 0.f;
-        for (int g = 0; g < groups; ++g) s += sm[g * pitch + c];
-        if (direct && !f32) gptr<T>(dst)[row * C + c] = f_to_elem<T>(s);
-        else gptr<float>(dst)[row * C + c] = s;
-    }
-}
-
 // With z the normalised branch (or the branch itself), W = residual_scale * scale * post_weight, B = residual_scale * scale * post_bias and
 // f = act(gate):   y = x + f (W z + B),   d = gradient of y (of the row's own dy and of h through the second norm)
 //   dbranch: q = f d W through the norm;    dgate = act'(gate) d (W z + B)
@@ -113,12 +77,9 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
                 *reinterpret_cast<float4*>(weights + which * pitch + p * plane + (k * at.lanes + at.lane) * 4) = make_float4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
         }
     };
-    auto get = [&](int which, int k, float* v) {
-#pragma unroll
-        for (int p = 0; p < V / 4; ++p) {
-            const float4 w = *reinterpret_cast<const float4*>(weights + which * pitch + p * plane + (k * at.lanes + at.lane) * 4);
-            v[4 * p] = w.x; v[4 * p + 1] = w.y; v[4 * p + 2] = w.z; v[4 * p + 3] = w.w;
-        }
+    auto get = [&](int which, int k, int p, float* v) {
+        const float4 w = *reinterpret_cast<const float4*>(weights + which * pitch + p * plane + (k * at.lanes + at.lane) * 4);
+        v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
     };
     enum { W_O = 0, W_B = 1, W_Y = BIAS ? 2 : 1 };
 #pragma unroll
@@ -169,31 +130,54 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
     clear(ao);
     clear(ao0);
 
-    // the branch's sums, each times its factor (see above), to row `to` of their destinations
-    auto leave_branch_sums = [&](long long to, long long gate_at) {
-#pragma unroll 1
-        for (int s = SUM_POST_W; s < SUM_COUNT; ++s) {
-            if (!plan.dst[s]) continue;
-            float v[K][V];
+    // A sum over the block's rows, one value per column, into array `which` of the LDS (in place of weights that are not read any more): the
+    // lanes' own columns side by side, several row groups added up in order.
+    auto collect = [&](const auto& acc, int which) {
+        float* out = weights + which * pitch;
+        if (groups == 1) {
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                float sc[V], w[V], b[V], g[V];
-                load_param_or<T, S::TINY>(a.scale, col[k], pf, left[k], 1.f, sc);
-                load_param_or<T, S::TINY>(a.post_weight, col[k], pf, left[k], 1.f, w);
-                load_param_or<T, S::TINY>(a.post_bias, col[k], pf, left[k], 0.f, b);
-                load_param_or<T, S::TINY>(GM == GM_CONST ? a.gate : 0, gate_at + col[k], gf, left[k], 1.f, g);
-                if (GM == GM_CONST && a.gate) {
-                    if (s == SUM_GATE) gate_slopes<V>(g, a.gate_act);
-                    else gate_values<V>(g, a.gate_act);
-                }
+            for (int k = 0; k < K; ++k)
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float p0 = BIAS ? ao0[BIAS ? k : 0][i] : 0.f;
-                    const float m = s == SUM_POST_W ? ao[k][i] : s == SUM_POST_B ? p0 : w[i] * ao[k][i] + b[i] * p0;
-                    v[k][i] = a.residual_scale * (s == SUM_SCALE ? 1.f : sc[i]) * g[i] * m;
-                }
+                for (int p = 0; p < V / 4; ++p)
+                    *reinterpret_cast<float4*>(out + col[k] + 4 * p) = make_float4(acc[k][4 * p], acc[k][4 * p + 1], acc[k][4 * p + 2], acc[k][4 * p + 3]);
+        } else {
+            __syncthreads();                         // the sum before has been read
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int i = 0; i < V; ++i) sm[at.group * pitch + col[k] + i] = acc[k][i];
+            __syncthreads();
+            for (int c = threadIdx.x; c < C; c += blockDim.x) {
+                float s = 0.f;
+                for (int g = 0; g < groups; ++g) s += sm[g * pitch + c];
+                out[c] = s;
             }
-            leave_sum<T, L, E>(v, plan.dst[s], to, C, (plan.direct >> s) & 1, s == SUM_GATE ? gf : pf, sm, at, groups);
+        }
+    };
+    auto leave = [&](int which, long long row, int c, float v, bool f32) {
+        const long long to = row * C + c;
+        if ((plan.direct >> which & 1) && !f32) gptr<T>(plan.dst[which])[to] = f_to_elem<T>(v);
+        else gptr<float>(plan.dst[which])[to] = v;
+    };
+    // the branch's sums, each times its factor (see above), to row `to` of their destinations: one column per thread
+    auto leave_branch_sums = [&](long long to, long long gate_at) {
+        if (!(plan.dst[SUM_POST_W] || plan.dst[SUM_POST_B] || plan.dst[SUM_SCALE] || plan.dst[SUM_GATE])) return;
+        __syncthreads();
+        collect(ao, W_O);
+        if (BIAS) collect(ao0, W_B);
+        __syncthreads();
+        for (int c = threadIdx.x; c < C; c += blockDim.x) {
+            const float p1 = weights[W_O * pitch + c], p0 = BIAS ? weights[W_B * pitch + c] : 0.f;
+            const float sc = a.residual_scale * (a.scale ? load_param1<T>(a.scale, c, pf) : 1.f);
+            const float g = GM == GM_CONST && a.gate ? load_param1<T>(a.gate, gate_at + c, gf) : 0.f;
+            const float f = GM == GM_CONST && a.gate ? gate_value(g, a.gate_act) : 1.f;
+            if (plan.dst[SUM_POST_W]) leave(SUM_POST_W, to, c, sc * f * p1, pf);
+            if (BIAS && plan.dst[SUM_POST_B]) leave(SUM_POST_B, to, c, sc * f * p0, pf);
+            if (plan.dst[SUM_SCALE] || plan.dst[SUM_GATE]) {
+                const float u = (a.post_weight ? load_param1<T>(a.post_weight, c, pf) : 1.f) * p1 + (BIAS && a.post_bias ? load_param1<T>(a.post_bias, c, pf) * p0 : 0.f);
+                if (plan.dst[SUM_SCALE]) leave(SUM_SCALE, to, c, a.residual_scale * f * u, pf);
+                if (plan.dst[SUM_GATE]) leave(SUM_GATE, to, c, sc * gate_slope(g, a.gate_act) * u, gf);
+            }
         }
     };
 
@@ -265,31 +249,30 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
 #pragma unroll
                 for (int k = 0; k < K; ++k) unpack16<T>(now.d[k], d[k]);
             } else {
-                float y[K][V], t[K][V], s2[2] = {0.f, 0.f};
+                float y[K][V], t[K][V], s2[2] = {0.f, 0.f}, wo[4], bo[4], wy[4];
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
                     unpack16<T>(now.x[k], y[k]);
                     unpack16<T>(now.t[k], t[k]);
-                    float wo[V], bo[V], wy[V];
-                    get(W_O, k, wo);
-                    if (BIAS) get(W_B, k, bo);
-                    if (WY_LDS) get(W_Y, k, wy);
-                    else {
-#pragma unroll
-                        for (int i = 0; i < V; ++i) wy[i] = wy_reg[WY_LDS ? 0 : k][i];
-                    }
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
+                        if (i % 4 == 0) {            // four columns at a time, to keep fewer weights in registers
+                            if (i) __builtin_amdgcn_sched_barrier(0);
+                            get(W_O, k, i / 4, wo);
+                            if (BIAS) get(W_B, k, i / 4, bo);
+                            if (WY_LDS) get(W_Y, k, i / 4, wy);
+                        }
+                        if (!WY_LDS) wy[i % 4] = wy_reg[WY_LDS ? 0 : k][i];
                         if (GM == GM_CONST) {
-                            y[k][i] = fmaf(wo[i], z[k][i], BIAS ? y[k][i] + bo[i] : y[k][i]);
+                            y[k][i] = fmaf(wo[i % 4], z[k][i], BIAS ? y[k][i] + bo[i % 4] : y[k][i]);
                         } else {
-                            const float u = BIAS ? fmaf(wo[i], z[k][i], bo[i]) : wo[i] * z[k][i];
+                            const float u = BIAS ? fmaf(wo[i % 4], z[k][i], bo[i % 4]) : wo[i % 4] * z[k][i];
                             y[k][i] = fmaf(GM == GM_ROW ? ft : f[GM == GM_VECTOR ? k : 0][i], u, y[k][i]);
                         }
                         y[k][i] = LAYER ? (y[k][i] - mu_y) * r_y : y[k][i] * r_y;
                         ay[k][i] = fmaf(t[k][i], y[k][i], ay[k][i]);
                         if (BIAS) ay0[BIAS ? k : 0][i] += t[k][i];
-                        t[k][i] *= wy[i];
+                        t[k][i] *= wy[i % 4];
                         if (LAYER) s2[0] += t[k][i];
                         s2[1] = fmaf(t[k][i], y[k][i], s2[1]);
                     }
@@ -324,9 +307,7 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
                 float s3[3] = {0.f, 0.f, 0.f};       // sums of q, q z and, per row, d B; q = d W, with the row's f put in after the sums
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
-                    float wo[V], bo[V];
-                    get(W_O, k, wo);
-                    if (BIAS) get(W_B, k, bo);
+                    float wo[4], bo[4];
                     if (GM == GM_VECTOR) {
                         float(&fk)[V] = f[GM == GM_VECTOR ? k : 0];
                         if (a.dgate) {
@@ -334,7 +315,13 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
                             load_param_or<T, S::TINY>(a.gate, row * a.gate_stride + col[k], gf, here ? left[k] : 0, 0.f, g);
                             gate_slopes<V>(g, a.gate_act);
 #pragma unroll
-                            for (int i = 0; i < V; ++i) g[i] *= d[k][i] * (BIAS ? fmaf(wo[i], z[k][i], bo[i]) : wo[i] * z[k][i]);
+                            for (int i = 0; i < V; ++i) {
+                                if (i % 4 == 0) {
+                                    get(W_O, k, i / 4, wo);
+                                    if (BIAS) get(W_B, k, i / 4, bo);
+                                }
+                                g[i] *= d[k][i] * (BIAS ? fmaf(wo[i % 4], z[k][i], bo[i % 4]) : wo[i % 4] * z[k][i]);
+                            }
                             if (here && left[k] > 0) store_param<T>(a.dgate, row * (long long)C + col[k], gf, left[k], g);
                         }
 #pragma unroll
@@ -342,11 +329,16 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
                     }
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
+                        if (i % 4 == 0) {
+                            if (i) __builtin_amdgcn_sched_barrier(0);
+                            get(W_O, k, i / 4, wo);
+                            if (BIAS) get(W_B, k, i / 4, bo);
+                        }
                         const float fd = GM == GM_ROW ? ft * d[k][i] : d[k][i];
                         ao[k][i] = fmaf(fd, z[k][i], ao[k][i]);
                         if (BIAS) ao0[BIAS ? k : 0][i] += fd;
-                        if (GM == GM_ROW && BIAS) s3[2] = fmaf(d[k][i], bo[i], s3[2]);
-                        d[k][i] *= wo[i];
+                        if (GM == GM_ROW && BIAS) s3[2] = fmaf(d[k][i], bo[i % 4], s3[2]);
+                        d[k][i] *= wo[i % 4];
                         if (LAYER) s3[0] += d[k][i];
                         s3[1] = fmaf(d[k][i], z[k][i], s3[1]);
                     }
@@ -377,14 +369,15 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
         clear(ao);
         clear(ao0);
     }
-    if (plan.dst[SUM_PRE_W]) leave_sum<T, L, E>(ay, plan.dst[SUM_PRE_W], blockIdx.x, C, (plan.direct >> SUM_PRE_W) & 1, pf, sm, at, groups);
-    if (BIAS && plan.dst[SUM_PRE_B]) {
-        float v[K][V];
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int i = 0; i < V; ++i) v[k][i] = ay0[BIAS ? k : 0][i];
-        leave_sum<T, L, E>(v, plan.dst[SUM_PRE_B], blockIdx.x, C, (plan.direct >> SUM_PRE_B) & 1, pf, sm, at, groups);
+    if (plan.dst[SUM_PRE_W] || plan.dst[SUM_PRE_B]) {
+        __syncthreads();
+        collect(ay, W_O);
+        if (BIAS) collect(ay0, W_B);
+        __syncthreads();
+        for (int c = threadIdx.x; c < C; c += blockDim.x) {
+            if (plan.dst[SUM_PRE_W]) leave(SUM_PRE_W, blockIdx.x, c, weights[W_O * pitch + c], pf);
+            if (BIAS && plan.dst[SUM_PRE_B]) leave(SUM_PRE_B, blockIdx.x, c, weights[W_B * pitch + c], pf);
+        }
     }
 }
 
