@@ -33,6 +33,27 @@ inline RowLaunch row_launch(int L, int E, int width) {
     return RowLaunch{w, r, 64 * w * r};
 }
 
+// How the rows are cut: segments = samples * parts, part p of a sample its rows [p * part_rows, (p + 1) * part_rows).  With a gate per sample
+// a segment ends with its sample, so that what the gate multiplies is constant over it; otherwise all rows are one "sample".
+struct RowCut {
+    int samples, parts;
+    long long sample_rows, part_rows;
+};
+// about `target` segments, each of at least min_steps steps of rpb rows where there are that many
+inline RowCut cut_rows(const FnetBlockNorm& a, int rpb, long long target, int min_steps) {
+    RowCut c;
+    const bool by_sample = a.gate_kind == FNET_GATE_SAMPLE;
+    c.samples = by_sample ? (int)(a.rows / a.tokens) : 1;
+    c.sample_rows = by_sample ? a.tokens : a.rows;
+    const long long steps = (c.sample_rows + rpb - 1) / rpb;
+    long long parts = target / c.samples;
+    if (parts > steps / min_steps) parts = steps / min_steps;
+    if (parts < 1) parts = 1;
+    c.part_rows = ((steps + parts - 1) / parts) * rpb;
+    c.parts = (int)((c.sample_rows + c.part_rows - 1) / c.part_rows);
+    return c;
+}
+
 // This thread's place: `lane` of row group `group`
 template <int L>
 struct RowPlace {
@@ -212,9 +233,10 @@ __device__ __forceinline__ void gate_slopes(float* g, int act) {
     }
 }
 
-// How the gate enters a kernel: constant over the rows that a block goes through (none, per channel, in the backward also per sample: part of
-// the weights), one value per row, or a row of values per row
-enum { GM_CONST = 0, GM_ROW = 1, GM_VECTOR = 2 };
+// How the gate enters a kernel: constant over a segment's rows (none, per channel, per sample: part of the weights), one value per row, or a
+// row of values per row.  (The forward has a gate per sample in an instance of its own: weights that change on the way cost it registers
+// that its waves in flight need.)
+enum { GM_CONST = 0, GM_ROW = 1, GM_VECTOR = 2, GM_SAMPLE = 3 };
 
 template <typename T, int L, int E>
 int fnet_block_norm_fwd_launch(const FnetBlockNorm& a, hipStream_t st);

@@ -10,8 +10,8 @@ struct BwdPlan {
     int direct;                  // bit i: dst[i] is the gradient, in its own type
     // the sums of the branch's side are left per segment (a sample's gate is part of them), those of the second norm per block; only with a
     // gate per sample does a block go through several segments
-    int samples, parts;          // segments = samples * parts: part p of a sample is its rows [p * part_rows, (p + 1) * part_rows)
-    long long sample_rows, part_rows;
+    RowCut cut;
+    int in_turn;                 // a sample's rows are dealt to its parts in turn; otherwise each part is a run of rows
 };
 
 // Waves per SIMD that the kernel is compiled for: 4 leave 128 registers to each; two more sums or a gate in registers do not fit those, and
@@ -181,11 +181,13 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
         }
     };
 
-    const int segments = plan.samples * plan.parts;
+    const int segments = plan.cut.samples * plan.cut.parts;
     for (int seg = blockIdx.x; seg < segments; seg += gridDim.x) {
-        const int sample = seg / plan.parts;
-        const long long first = sample * plan.sample_rows + (seg - sample * plan.parts) * plan.part_rows;
-        const long long end = min(first + plan.part_rows, (sample + 1) * plan.sample_rows);
+        const int sample = seg / plan.cut.parts;
+        const long long begin = sample * plan.cut.sample_rows, part = seg - sample * plan.cut.parts;
+        const long long first = begin + part * (plan.in_turn ? groups : plan.cut.part_rows);
+        const long long end = min(plan.in_turn ? begin + plan.cut.sample_rows : first + plan.cut.part_rows, begin + plan.cut.sample_rows);
+        const long long stride = plan.in_turn ? (long long)plan.cut.parts * groups : groups;
         const long long sample_gate = a.gate_kind == FNET_GATE_SAMPLE ? (long long)sample * a.gate_stride : 0;
         load_branch_side(sample_gate);
         struct Row {
@@ -223,7 +225,7 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
             }
         };
         // several waves to a row go through the barriers of its sums together: a block's groups take the same number of steps
-        for (long long step = first; step < end; step += groups) {
+        for (long long step = first; step < end; step += stride) {
             const long long row = S::row(step + at.group);
             const bool here = row < end;
             if (!S::WAVES && !here) break;
