@@ -198,16 +198,16 @@ __device__ __forceinline__ void store_param(uint64_t p, long long at, bool f32, 
 }
 
 // act(g) and its derivative of a chunk; the choice is uniform, so it stands outside the loops.  Both derivatives are written with
-// e = exp(-|g|) (or its square), which keeps them exact where act(g) is within a rounding of 1.
+// e = exp(-|g|) (or its square), which keeps them exact where act(g) is within a rounding of 1.  v_rcp_f32 is good for one unit in the last place.
 __device__ __forceinline__ float gate_value(float g, int act) {
-    if (act == FNET_GATE_SIGMOID) return 1.f / (1.f + __expf(-g));
+    if (act == FNET_GATE_SIGMOID) return __builtin_amdgcn_rcpf(1.f + __expf(-g));
     if (act == FNET_GATE_TANH) return tanhf(g);
     return g;
 }
 __device__ __forceinline__ float gate_slope(float g, int act) {
     if (act == FNET_GATE_IDENTITY) return 1.f;
-    const float e = __expf(act == FNET_GATE_SIGMOID ? -fabsf(g) : -2.f * fabsf(g)), d = 1.f + e;
-    return (act == FNET_GATE_SIGMOID ? e : 4.f * e) / (d * d);
+    const float e = __expf(act == FNET_GATE_SIGMOID ? -fabsf(g) : -2.f * fabsf(g)), r = __builtin_amdgcn_rcpf(1.f + e);
+    return (act == FNET_GATE_SIGMOID ? e : 4.f * e) * r * r;
 }
 template <int V>
 __device__ __forceinline__ void gate_values(float* g, int act) {
