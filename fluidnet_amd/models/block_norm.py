@@ -19,15 +19,17 @@ x and branch: [..., C], fp32, bf16 or fp16, 1 <= C <= 16384, any number of rows 
 spaced, or the operand is copied first; slices of the last axis are taken as they are.  Weights, biases and scale: [C], all of them in fp32 or
 all in x's type.  gate, in fp32 or x's type: like x (a value per element), [..., 1] (per token), [B, 1, .., 1, C] for x [B, .., C] (per sample)
 or [C] (per channel); gate_act "identity", "sigmoid" or "tanh".  A NaN or infinity stays in its row (and in the sums over rows).
-There is no CPU fallback.
+There is no CPU fallback, and no second derivative (asking for one raises).
 """
 from __future__ import annotations
 
+import ctypes
 import struct
 from typing import Literal, Optional, Tuple
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from ..engine import runtime as rt
 from ..engine.elements import ELEM
@@ -45,7 +47,7 @@ _ARGS = struct.Struct("=7q8i2f22Qq")
 
 class _Spec:
     """What a call is, apart from its tensors."""
-    __slots__ = ("rows", "tokens", "width", "param_dtype", "gate_dtype", "pre", "post", "gate_kind", "samples", "fixed")
+    __slots__ = ("rows", "tokens", "width", "param_dtype", "gate_dtype", "pre", "post", "gate_kind", "fixed")
 
 
 def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
@@ -133,14 +135,13 @@ def _spec(x, branch, gate, scale, pw, pb, nw, nb, kind, post, pre, gate_act, res
         seen = _param_type("pre_weight", nw, C, x, seen)
     if nb is not None:
         seen = _param_type("pre_bias", nb, C, x, seen)
-    gate_kind, gate_dtype, s.tokens, s.samples = _NONE, 0, rows, 1
+    gate_kind, gate_dtype, s.tokens = _NONE, 0, rows
     if gate is not None:
         if gate.get_device() != x.get_device() or (gate.dtype is not torch.float32 and gate.dtype is not x.dtype):
             raise ValueError(f"gate must be float32 or {x.dtype} on {x.device} (got {gate.dtype} on {gate.device})")
         gate_kind, gate_dtype = _gate_kind(gate, x), ELEM[gate.dtype]
         if gate_kind == _SAMPLE and rows:
-            s.samples = shape[0]
-            s.tokens = rows // s.samples
+            s.tokens = rows // shape[0]
             if s.tokens == 1:                 # a row of values per row
                 gate_kind = _ELEMENT
     s.gate_kind, s.pre, s.post = gate_kind, bool(pre), bool(post)
@@ -204,15 +205,6 @@ def _forward(s: _Spec, x, branch, gate, scale, pw, pb, nw, nb, keep: bool):
     return y, h, stats
 
 
-def _workspace(s: _Spec, sums: int) -> int:
-    """Bytes that hold the partial sums of a backward with so many gradients over rows (fnet_block_norm_workspace gives the exact number): at
-    most a row per four rows of the operands, and per block that fits the GPU or sample."""
-    C = s.width
-    blocks = 1024 if C <= 2048 else 256 * max(1, 16 // -(-C // 512))
-    rows = min(s.rows, max(blocks, s.samples))
-    return sums * (4 * C * rows + 16)
-
-
 class _BlockNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, s, x, branch, gate, scale, pw, pb, nw, nb):
@@ -223,6 +215,7 @@ class _BlockNormFn(torch.autograd.Function):
         return y, h
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dh):
         s = ctx.s
         x, branch, gate, scale, pw, pb, nw, nb, stats = ctx.saved_tensors
@@ -235,19 +228,19 @@ class _BlockNormFn(torch.autograd.Function):
         dx = None if not nx else make(x, memory_format=_DENSE) if with_h else dy
         db = make(branch, memory_format=_DENSE) if nbr and branch is not None else None
         dg = make(gate, memory_format=_DENSE) if ng and gate is not None else None
-        sums = 0 if dg is None else 1
+        sums = dg is not None
         dsc = dpw = dpb = dnw = dnb = None
         if nsc and scale is not None:
-            dsc, sums = make(scale, memory_format=_DENSE), sums + 1
+            dsc, sums = make(scale, memory_format=_DENSE), True
         if npw and pw is not None:
-            dpw, sums = make(pw, memory_format=_DENSE), sums + 1
+            dpw, sums = make(pw, memory_format=_DENSE), True
         if npb and pb is not None:
-            dpb, sums = make(pb, memory_format=_DENSE), sums + 1
+            dpb, sums = make(pb, memory_format=_DENSE), True
         norm = make if with_h else torch.zeros_like
         if nnw and nw is not None:
-            dnw, sums = norm(nw, memory_format=_DENSE), sums + 1
+            dnw, sums = norm(nw, memory_format=_DENSE), True
         if nnb and nb is not None:
-            dnb, sums = norm(nb, memory_format=_DENSE), sums + 1
+            dnb, sums = norm(nb, memory_format=_DENSE), True
         if s.rows and (with_h or db is not None or dg is not None or sums):
             strides, ptrs, _keep = _operands(s, x, branch, gate, scale, pw, pb, nw, nb)
             py = ys = ph = hs = px = p0 = p1 = 0
@@ -260,11 +253,16 @@ class _BlockNormFn(torch.autograd.Function):
                 px = 0 if dx is None else dx.data_ptr()
                 p0 = 0 if dnw is None else dnw.data_ptr()
                 p1 = 0 if dnb is None else dnb.data_ptr()
-            n = _workspace(s, sums) if sums else 0
+            a = (s.rows, s.tokens, *strides, ys, hs, *s.fixed, *ptrs, 0, 0, 0 if stats is None else stats.data_ptr(), py, ph, px,
+                 0 if db is None else db.data_ptr(), 0 if dg is None else dg.data_ptr(), 0 if dsc is None else dsc.data_ptr(),
+                 0 if dpw is None else dpw.data_ptr(), 0 if dpb is None else dpb.data_ptr(), p0, p1)
+            n = 0
+            if sums:                              # partial sums of what is summed over rows
+                need = ctypes.c_int64()
+                rt.check(rt.lib().fnet_block_norm_workspace(_ARGS.pack(*a, 0, 0), ctypes.byref(need)), "fnet_block_norm_workspace")
+                n = need.value
             ws = x.new_empty(n, dtype=torch.uint8) if n else None
-            a = _ARGS.pack(s.rows, s.tokens, *strides, ys, hs, *s.fixed, *ptrs, 0, 0, 0 if stats is None else stats.data_ptr(), py, ph, px,
-                           0 if db is None else db.data_ptr(), 0 if dg is None else dg.data_ptr(), 0 if dsc is None else dsc.data_ptr(),
-                           0 if dpw is None else dpw.data_ptr(), 0 if dpb is None else dpb.data_ptr(), p0, p1, 0 if ws is None else ws.data_ptr(), n)
+            a = _ARGS.pack(*a, 0 if ws is None else ws.data_ptr(), n)
             rt.call_on(x, "fnet_block_norm_bwd", a)
         return None, dx, db, dg, dsc, dpw, dpb, dnw, dnb
 

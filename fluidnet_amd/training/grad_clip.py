@@ -64,9 +64,10 @@ class TensorList:
             k, t = next((k, t) for k, t in enumerate(tensors) if t.dtype not in ELEM or t.get_device() != device)
             raise ValueError(f"{what} {k} must be a float32, bfloat16 or float16 tensor on {self.first.device} (got {t.dtype} on {t.device})")
         strided = []
-        if not all(map(_contiguous, tensors)):
+        self.contiguous = all(map(_contiguous, tensors))
+        if not self.contiguous:
             tensors, types, strided = self._split(tensors, what)
-        self.n, self.n_strided = len(tensors), len(strided)
+        self.n, self.n_strided, self.types = len(tensors), len(strided), types
         self._keep = (array("Q", map(_address, tensors)), array("q", map(_numel, tensors)), array("i", map(ELEM.__getitem__, types)), b"".join(strided))
         self.ptrs, self.numels, self.codes = (a.buffer_info()[0] for a in self._keep[:3])
         self.strided = ctypes.cast(ctypes.c_char_p(self._keep[3]), ctypes.c_void_p) if strided else None
@@ -86,6 +87,8 @@ class TensorList:
                 strided.append(_STRIDED.pack(t.data_ptr(), ELEM[t.dtype], len(axes), *(n for _, n in axes), *pad, *(st for st, _ in axes), *pad))
             else:
                 dense.append(t)
+        if len(set(strided)) != len(strided):
+            raise ValueError(f"a {what} appears twice")
         return dense, [t.dtype for t in dense], strided
 
     def args(self):
@@ -141,7 +144,8 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """Scales the gradients of `parameters` in place by min(1, max_norm / (norm + 1e-6)) and returns the norm that they had (0-dim, fp32, on
     their device).  Parameters without a gradient are passed over.  A norm that is not finite scales as torch does (gradients become 0 or NaN),
-    or raises with error_if_nonfinite=True, which waits for the GPU.  Gradients that share memory are refused."""
+    or raises with error_if_nonfinite=True, which waits for the GPU.  Dense gradients that share memory are refused, and a strided
+    one that appears twice."""
     kind, max_norm = _norm_kind(norm_type), _max_norm(max_norm)
     grads = _grads(parameters)
     if not grads:

@@ -135,10 +135,10 @@ def clip_adam_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     if any(masters[k] is None for k in low):
         raise ValueError(f"parameter {next(k for k in low if masters[k] is None)} is not float32 and needs an fp32 master")
     state = exp_avgs + exp_avg_sqs + [masters[k] for k in low]
-    numels = list(map(_numel, grads))
-    if not (types == list(map(_dtype, grads)) and set(map(_dtype, state)) == {f32} and set(map(_device, params + state)) == {dev}
+    numels = list(map(_numel, params))
+    if not (lst.contiguous and types == lst.types and set(map(_dtype, state)) == {f32} and set(map(_device, params + state)) == {dev}
             and list(map(_shape, params)) == list(map(_shape, grads)) and list(map(_numel, state)) == numels + numels + [numels[k] for k in low]
-            and all(map(_contiguous, params + grads + state))):
+            and all(map(_contiguous, params + state))):
         _check_layouts(params, grads, exp_avgs, exp_avg_sqs, masters)
     for name, t, count in (("clock", clock, 3),) + ((("lr", lr, 1),) if isinstance(lr, torch.Tensor) else ()):
         if t.dtype is not torch.float64 or t.numel() != count or t.get_device() != dev or not t.is_contiguous():

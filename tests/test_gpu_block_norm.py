@@ -119,6 +119,45 @@ def test_rows(shape):
         assert g.shape == d[n].shape and g.dtype == d[n].dtype and not g.any(), n
 
 
+@pytest.mark.parametrize("width,rows", [(1300, 6000), (1100, 9000), (640, 6000), (2049, 3000), (4507, 1500), (6000, 1200), (9000, 600), (500, 9000), (40, 40_000)])
+def test_many_rows(width, rows):
+    """More rows than the GPU holds blocks of, for rows of 2, 3, 5, 9, 12 and 16 waves: the partial sums of every block."""
+    t, dy, dh = operands((rows, width), BF16, gate="channel", bias=True, seed=width)
+    both(t, dy, dh, kind="layer", act="sigmoid")
+    t, dy, dh = operands((10, rows // 10, width), F32 if width < 2000 else F16, gate="sample", scale=True, seed=width)
+    both(t, dy, dh, act="tanh")
+
+
+def test_no_second_derivative():
+    t, dy, dh = operands((3, 16), F32)
+    d = gpu(t, True)
+    y, h = call(d, "rms", "identity", 1.0, 1e-6)
+    g, = torch.autograd.grad([y, h], [d["x"]], [dy.cuda().requires_grad_(True), dh.cuda()], create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+
+
+def test_capture_of_a_shape_that_never_ran():
+    """The first call of a shape asks the runtime how many blocks fit, also while a graph is captured."""
+    t, dy, dh = operands((700, 3333), BF16, gate="channel", bias=True)
+    d = gpu(t, True)
+    dyg, dhg = dy.cuda(), dh.cuda()
+    names = [n for n in ref.NAMES if n in d]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, h = call(d, "layer", "tanh", 1.0, 1e-6)
+        out = [y, h, *torch.autograd.grad([y, h], [d[n] for n in names], [dyg, dhg])]
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        y, h = call(gpu(t, True), "layer", "tanh", 1.0, 1e-6)
+        assert torch.equal(out[0], y) and torch.equal(out[1], h)
+        want, tol = ref.reference(t, "layer", "tanh", 1.0, 1e-6, dy, dh), ref.tolerance(t, "layer", "tanh", 1.0, 1e-6, dy, dh)
+        for n, v in zip(names, out[2:]):
+            ref.check(v, want["d_" + n], tol["d_" + n], n)
+
+
 def test_one_gradient_at_a_time():
     """Only dy, only dh, and one operand that needs a gradient: every other one is not computed, the one is as always."""
     t, dy, dh = operands((9, 70), F32, gate="element", scale=True, bias=True)

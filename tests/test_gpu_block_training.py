@@ -49,7 +49,7 @@ def _same_in_64_bits(net, x, weight):
                         **j(0, "scale", "post_weight", "post_bias", "pre_weight", "pre_bias")}, "layer", "sigmoid", 1.0, 1e-6)
     v, h = ref.forward({"x": v, "branch": lin("blocks.1", h), "post": False, "pre": True, **j(1, "gate", "pre_weight")}, "rms", "tanh", 1.0, 1e-6)
     loss = (lin("head", h).permute(0, 3, 1, 2) * weight.cpu().double()).sum()
-    return float(loss), dict(zip(p, torch.autograd.grad(loss, list(p.values()))))
+    return float(loss.detach()), dict(zip(p, torch.autograd.grad(loss, list(p.values()))))
 
 
 def test_gradients_clip_and_step_together():

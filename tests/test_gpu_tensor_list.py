@@ -123,6 +123,9 @@ def test_refusals():
     with pytest.raises(FluidNetHipError, match="share memory"):
         clip_grad_norm_(_params([t[:6], t[5:]]), 1.0)
     _check_norm(total_grad_norm([t + 1, t + 1]), [t + 1, t + 1], 2.0)
+    wide = torch.ones(6, 4, device="cuda")
+    with pytest.raises(ValueError, match="twice"):
+        clip_grad_norm_(_params([wide[:, 1], wide[:, 1]]), 1.0)
     for bad in (torch.zeros(3, device="cuda", dtype=torch.float64), torch.zeros(3, device="cuda", dtype=torch.int32), torch.zeros(3),
                 torch.zeros(1, 4, device="cuda").expand(3, 4), torch.zeros([3] * 7, device="cuda").permute(6, 5, 4, 3, 2, 1, 0)[::2, ::2, ::2, ::2, ::2, ::2, ::2]):
         with pytest.raises((ValueError, RuntimeError)):
@@ -315,6 +318,19 @@ def test_master_follows_a_parameter_written_from_outside():
     p.grad = torch.ones_like(p)
     opt.step()
     assert float((opt._w[0] + 2.0).abs().max()) < 4e-3
+
+
+def test_optimizer_takes_gradients_of_any_layout():
+    """A gradient that is a slice of a wider buffer, or transposed, gives the step of its contiguous copy."""
+    g = torch.Generator().manual_seed(8)
+    a, b = ([torch.nn.Parameter(torch.randn(6, 5, generator=torch.Generator().manual_seed(1)).cuda()) for _ in range(2)] for _ in range(2))
+    wide = torch.randn(6, 12, generator=g).cuda()
+    a[0].grad, a[1].grad = wide[:, 2:7], torch.randn(5, 6, generator=g).cuda().t()
+    for p, q in zip(a, b):
+        q.grad = p.grad.contiguous()
+    for ps in (a, b):
+        ClipAdam(ps, 1e-2, max_norm=0.1).step()
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
 def test_graphs_of_clip_and_step():
