@@ -1,5 +1,7 @@
 // Shared by the forward and the backward of the norms around a residual block (fnet_block_norm*.hip).
 #pragma once
+#include <algorithm>
+
 #include "fnet_vec.h"
 
 // How rows lie on lanes.  A row is held in registers from its one load to its last store, E elements a lane in chunks of 16 bytes: lane l of
@@ -39,7 +41,7 @@ struct RowCut {
     int samples, parts;
     long long sample_rows, part_rows;
 };
-// about `target` segments, each of at least min_steps steps of rpb rows where there are that many
+// about `target` segments, each of at least min_steps steps of rpb rows where there are that many for 256 of them
 inline RowCut cut_rows(const FnetBlockNorm& a, int rpb, long long target, int min_steps) {
     RowCut c;
     const bool by_sample = a.gate_kind == FNET_GATE_SAMPLE;
@@ -47,7 +49,8 @@ inline RowCut cut_rows(const FnetBlockNorm& a, int rpb, long long target, int mi
     c.sample_rows = by_sample ? a.tokens : a.rows;
     const long long steps = (c.sample_rows + rpb - 1) / rpb;
     long long parts = target / c.samples;
-    if (parts > steps / min_steps) parts = steps / min_steps;
+    const long long fill = std::min(steps, (long long)(255 + c.samples) / c.samples);
+    parts = std::min(parts, std::max(steps / min_steps, fill));
     if (parts < 1) parts = 1;
     c.part_rows = ((steps + parts - 1) / parts) * rpb;
     c.parts = (int)((c.sample_rows + c.part_rows - 1) / c.part_rows);

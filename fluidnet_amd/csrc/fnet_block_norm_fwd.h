@@ -1,7 +1,5 @@
 // The forward kernel of the norms around a residual block, for one operand type; fnet_block_norm_{f32,bf16,f16}.hip instantiate it.
 #pragma once
-#include <algorithm>
-
 #include "fnet_block_norm.h"
 
 namespace {
