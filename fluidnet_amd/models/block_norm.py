@@ -205,6 +205,60 @@ def _forward(s: _Spec, x, branch, gate, scale, pw, pb, nw, nb, keep: bool):
     return y, h, stats
 
 
+def _backward(ctx, dy, dh):
+    s = ctx.s
+    x, branch, gate, scale, pw, pb, nw, nb, stats = ctx.saved_tensors
+    _, nx, nbr, ng, nsc, npw, npb, nnw, nnb = ctx.needs_input_grad
+    if dy is None and dh is None:
+        return (None,) * 9
+    make = torch.empty_like if s.rows else torch.zeros_like
+    with_h = dh is not None
+    # without a gradient of h, the gradient of x is that of y
+    dx = None if not nx else make(x, memory_format=_DENSE) if with_h else dy
+    db = make(branch, memory_format=_DENSE) if nbr and branch is not None else None
+    dg = make(gate, memory_format=_DENSE) if ng and gate is not None else None
+    sums = dg is not None
+    dsc = dpw = dpb = dnw = dnb = None
+    if nsc and scale is not None:
+        dsc, sums = make(scale, memory_format=_DENSE), True
+    if npw and pw is not None:
+        dpw, sums = make(pw, memory_format=_DENSE), True
+    if npb and pb is not None:
+        dpb, sums = make(pb, memory_format=_DENSE), True
+    norm = make if with_h else torch.zeros_like
+    if nnw and nw is not None:
+        dnw, sums = norm(nw, memory_format=_DENSE), True
+    if nnb and nb is not None:
+        dnb, sums = norm(nb, memory_format=_DENSE), True
+    if s.rows and (with_h or db is not None or dg is not None or sums):
+        strides, ptrs, _keep = _operands(s, x, branch, gate, scale, pw, pb, nw, nb)
+        py = ys = ph = hs = px = p0 = p1 = 0
+        if dy is not None:
+            dy, ys = _rows(dy)
+            py = dy.data_ptr()
+        if with_h:
+            dh, hs = _rows(dh)
+            ph = dh.data_ptr()
+            px = 0 if dx is None else dx.data_ptr()
+            p0 = 0 if dnw is None else dnw.data_ptr()
+            p1 = 0 if dnb is None else dnb.data_ptr()
+        a = (s.rows, s.tokens, *strides, ys, hs, *s.fixed, *ptrs, 0, 0, 0 if stats is None else stats.data_ptr(), py, ph, px,
+             0 if db is None else db.data_ptr(), 0 if dg is None else dg.data_ptr(), 0 if dsc is None else dsc.data_ptr(),
+             0 if dpw is None else dpw.data_ptr(), 0 if dpb is None else dpb.data_ptr(), p0, p1)
+        n = 0
+        if sums:                              # partial sums of what is summed over rows
+            need = ctypes.c_int64()
+            rt.check(rt.lib().fnet_block_norm_workspace(_ARGS.pack(*a, 0, 0), ctypes.byref(need)), "fnet_block_norm_workspace")
+            n = need.value
+        ws = x.new_empty(n, dtype=torch.uint8) if n else None
+        a = _ARGS.pack(*a, 0 if ws is None else ws.data_ptr(), n)
+        rt.call_on(x, "fnet_block_norm_bwd", a)
+    return None, dx, db, dg, dsc, dpw, dpb, dnw, dnb
+
+
+_backward_once = once_differentiable(_backward)
+
+
 class _BlockNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, s, x, branch, gate, scale, pw, pb, nw, nb):
@@ -215,56 +269,9 @@ class _BlockNormFn(torch.autograd.Function):
         return y, h
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dh):
-        s = ctx.s
-        x, branch, gate, scale, pw, pb, nw, nb, stats = ctx.saved_tensors
-        _, nx, nbr, ng, nsc, npw, npb, nnw, nnb = ctx.needs_input_grad
-        if dy is None and dh is None:
-            return (None,) * 9
-        make = torch.empty_like if s.rows else torch.zeros_like
-        with_h = dh is not None
-        # without a gradient of h, the gradient of x is that of y
-        dx = None if not nx else make(x, memory_format=_DENSE) if with_h else dy
-        db = make(branch, memory_format=_DENSE) if nbr and branch is not None else None
-        dg = make(gate, memory_format=_DENSE) if ng and gate is not None else None
-        sums = dg is not None
-        dsc = dpw = dpb = dnw = dnb = None
-        if nsc and scale is not None:
-            dsc, sums = make(scale, memory_format=_DENSE), True
-        if npw and pw is not None:
-            dpw, sums = make(pw, memory_format=_DENSE), True
-        if npb and pb is not None:
-            dpb, sums = make(pb, memory_format=_DENSE), True
-        norm = make if with_h else torch.zeros_like
-        if nnw and nw is not None:
-            dnw, sums = norm(nw, memory_format=_DENSE), True
-        if nnb and nb is not None:
-            dnb, sums = norm(nb, memory_format=_DENSE), True
-        if s.rows and (with_h or db is not None or dg is not None or sums):
-            strides, ptrs, _keep = _operands(s, x, branch, gate, scale, pw, pb, nw, nb)
-            py = ys = ph = hs = px = p0 = p1 = 0
-            if dy is not None:
-                dy, ys = _rows(dy)
-                py = dy.data_ptr()
-            if with_h:
-                dh, hs = _rows(dh)
-                ph = dh.data_ptr()
-                px = 0 if dx is None else dx.data_ptr()
-                p0 = 0 if dnw is None else dnw.data_ptr()
-                p1 = 0 if dnb is None else dnb.data_ptr()
-            a = (s.rows, s.tokens, *strides, ys, hs, *s.fixed, *ptrs, 0, 0, 0 if stats is None else stats.data_ptr(), py, ph, px,
-                 0 if db is None else db.data_ptr(), 0 if dg is None else dg.data_ptr(), 0 if dsc is None else dsc.data_ptr(),
-                 0 if dpw is None else dpw.data_ptr(), 0 if dpb is None else dpb.data_ptr(), p0, p1)
-            n = 0
-            if sums:                              # partial sums of what is summed over rows
-                need = ctypes.c_int64()
-                rt.check(rt.lib().fnet_block_norm_workspace(_ARGS.pack(*a, 0, 0), ctypes.byref(need)), "fnet_block_norm_workspace")
-                n = need.value
-            ws = x.new_empty(n, dtype=torch.uint8) if n else None
-            a = _ARGS.pack(*a, 0 if ws is None else ws.data_ptr(), n)
-            rt.call_on(x, "fnet_block_norm_bwd", a)
-        return None, dx, db, dg, dsc, dpw, dpb, dnw, dnb
+        # with create_graph the gradients are marked as having no derivative of their own; without it nobody can ask for one
+        return _backward_once(ctx, dy, dh) if torch.is_grad_enabled() else _backward(ctx, dy, dh)
 
 
 def _run(s: _Spec, *operands):
