@@ -178,6 +178,8 @@ class ClipAdam:
         self.params: List[torch.Tensor] = list(params)
         if not self.params:
             raise ValueError("ClipAdam got no parameters")
+        if not all(isinstance(p, torch.Tensor) for p in self.params):
+            raise TypeError("ClipAdam takes parameters, not groups of them")
         if len({id(p) for p in self.params}) != len(self.params):
             raise ValueError("a parameter appears twice")
         self.max_norm = None if max_norm is None else _max_norm(max_norm)

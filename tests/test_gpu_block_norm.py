@@ -103,6 +103,17 @@ def test_parts(post, pre, branch, weights, kind):
         both(t, dy, dh, kind=kind, act="sigmoid")
 
 
+def test_a_single_vector():
+    """x of one axis: one row, with a gate per element or one value."""
+    for gate, width in (("element", 70), ("token", 300)):
+        t, dy, dh = operands((width,), BF16, gate="element", bias=True)
+        if gate == "token":
+            t["gate"] = t["gate"][:1]
+        both(t, dy, dh, kind="layer", act="tanh")
+        both(t, dy, dh, on=lambda t: {k: v.cuda().repeat_interleave(2)[::2].detach().requires_grad_(True) if isinstance(v, torch.Tensor) else v
+                                      for k, v in t.items()})
+
+
 @pytest.mark.parametrize("shape", [(0, 64), (4, 0, 1024), (0, 3, 8), (1, 1), (1, 4096), (8192, 8), (3, 1, 16), (17, 1, 33), (1100, 2, 40), (2100, 3, 24)],
                          ids=str)
 def test_rows(shape):

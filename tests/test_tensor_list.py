@@ -35,6 +35,7 @@ def test_nothing_to_clip():
     (ValueError, "max_norm", lambda: clip_grad_norm_([_param()], float("nan"))),
     (ValueError, "no parameters", lambda: ClipAdam([], 1e-3)),
     (ValueError, "twice", lambda: ClipAdam([_param()] * 2, 1e-3)),
+    (TypeError, "groups", lambda: ClipAdam([{"params": [_param()]}], 1e-3)),
     (ValueError, "equally long", lambda: clip_adam_([], [], [], [], torch.zeros(3), lr=1.0)),
     (ValueError, "equally long", lambda: clip_adam_([_param()], [], [], [], torch.zeros(3), lr=1.0)),
     (ValueError, "betas", lambda: clip_adam_(*[[_param()]] * 4, torch.zeros(3), lr=1.0, betas=(1.0, 0.9))),
