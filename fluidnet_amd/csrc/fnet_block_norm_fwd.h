@@ -192,9 +192,10 @@ int fnet_block_norm_fwd_launch(const FnetBlockNorm& a, hipStream_t st) {
 #undef FNET_FWD
     // one block for each that the GPU holds: a second round would run with part of the GPU idle
     int most = fnet_resident_blocks(kernel, rl.threads, 0, 256 * 1024 / rl.threads);
-    // rows up to 2048: 24 waves a CU are enough, and 32 fetch more lines than they find again (16384 x 2048 with a gate per token 56 us with 32,
-    // 47 with 24; 131072 x 256 with biases 55 and 49); blocks of wider rows would leave room unused (4096 x 8192: 45 and 49)
-    if (rl.threads <= 256) most = std::min(most, 256 * 24 * 64 / rl.threads);
+    // ... up to 24 waves a CU, but two blocks.  30 M bf16 elements, rms, none / with a gate per token: 4096 wide 41 / 42 us with three blocks of 8
+    // waves, 43 / 51 with four; 4608 wide 41 / 46 with two of 9, 42 / 55 with three; 2304 wide 41 / 43 with four of 5, 49 / 52 with six; 8192
+    // wide 50 / 55 with one of 16, 42 / 60 with two.
+    most = std::min(most, 256 * std::max(2, 24 * 64 / rl.threads));
     RowCut cut = cut_rows(a, rl.rpb, most, 1);
     FnetBlockNorm arg = a;
     RowLaunch r = rl;
