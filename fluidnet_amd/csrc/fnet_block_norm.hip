@@ -1,5 +1,6 @@
 // Norms around a residual block: argument checks, the cut of the rows, the sum of a backward's partial sums and the C entries.  The two large
 // kernels are in fnet_block_norm_fwd.h / fnet_block_norm_bwd.h, compiled once per operand type (fnet_block_norm_{f32,bf16,f16}.hip).
+#include <algorithm>
 #include <mutex>
 
 #include "fnet_block_norm_bwd.h"
@@ -25,12 +26,24 @@ int fnet_resident_blocks(const void* kernel, int threads, size_t lds, int otherw
         Known& k = known[h & 1023];
         if (k.kernel == kernel && k.threads == threads && k.lds == lds && k.device == dev) return k.blocks;
         if (k.kernel) continue;
-        int per_cu = 0, cus = 0;
-        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, threads, lds) != hipSuccess || per_cu < 1 ||
-            hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus < 1) {
+        // What a CU holds, from the kernel's registers and LDS: hipOccupancyMaxActiveBlocksPerMultiprocessor names more where the waves of a block
+        // are no multiple of four, and blocks too many run one after the rest.  Measured, 5 waves take
+        // the room of 8 (bf16 backward, 13020 x 2304: 112 us with three blocks a CU, 90 with two; forward, 10653 x 2816 with a gate per token:
+        // 67 and 54).  Three waves a block pack better in some kernels: 25000 x 1200 layer norms with biases 149 -> 113, with a gate per element
+        // and no biases 144 -> 168.
+        hipFuncAttributes attr;
+        int cus = 0, shared = 0;
+        if (hipFuncGetAttributes(&attr, kernel) != hipSuccess || attr.numRegs < 1 ||
+            hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus < 1 ||
+            hipDeviceGetAttribute(&shared, hipDeviceAttributeMaxSharedMemoryPerMultiprocessor, dev) != hipSuccess || shared < 1) {
             (void)hipGetLastError();
             return otherwise;
         }
+        const int waves = std::min(8, 512 / ((attr.numRegs + 7) / 8 * 8)), per_simd = (threads / 64 + 3) / 4;
+        const size_t bytes = attr.sharedSizeBytes + lds;
+        int per_cu = waves / per_simd;
+        if (bytes) per_cu = std::min(per_cu, (int)(shared / bytes));
+        per_cu = std::max(per_cu, 1);
         if (count < 1000) {
             ++count;
             k = Known{kernel, threads, dev, lds, per_cu * cus};
