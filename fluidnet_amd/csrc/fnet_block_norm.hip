@@ -27,10 +27,9 @@ int fnet_resident_blocks(const void* kernel, int threads, size_t lds, int otherw
         if (k.kernel == kernel && k.threads == threads && k.lds == lds && k.device == dev) return k.blocks;
         if (k.kernel) continue;
         // What a CU holds, from the kernel's registers and LDS: hipOccupancyMaxActiveBlocksPerMultiprocessor names more where the waves of a block
-        // are no multiple of four, and blocks too many run one after the rest.  Measured, 5 waves take
-        // the room of 8 (bf16 backward, 13020 x 2304: 112 us with three blocks a CU, 90 with two; forward, 10653 x 2816 with a gate per token:
-        // 67 and 54).  Three waves a block pack better in some kernels: 25000 x 1200 layer norms with biases 149 -> 113, with a gate per element
-        // and no biases 144 -> 168.
+        // are no multiple of four, and blocks too many run one after the rest.  Measured, 5 waves take the room of 8 (bf16 backward, 13020 x
+        // 2304: 112 us with three blocks a CU, 90 with two; forward, 10653 x 2816 with a gate per token: 67 and 54).  Three waves a block pack
+        // better in some kernels: 25000 x 1200 layer norms with biases 149 -> 113, with a gate per element and no biases 144 -> 168.
         hipFuncAttributes attr;
         int cus = 0, shared = 0;
         if (hipFuncGetAttributes(&attr, kernel) != hipSuccess || attr.numRegs < 1 ||
@@ -162,7 +161,7 @@ void bwd_shape(const FnetBlockNorm& a, int L, int E, int most, BwdShape* out) {
     const uint64_t want[SUM_COUNT] = {a.dpre_weight, a.dpre_bias, a.dpost_weight, a.dpost_bias, a.dscale, out->gm == GM_CONST ? a.dgate : 0};
     for (int s = 0; s < SUM_COUNT; ++s) {
         if (!want[s]) continue;
-        const long long rows = s >= SUM_POST_W ? segments : out->blocks;
+        const long long rows = s == SUM_GATE ? segments : out->blocks;
         if (s == SUM_GATE && by_sample ? p.cut.parts == 1 : rows == 1) {
             p.direct |= 1 << s;
             p.dst[s] = want[s];
@@ -207,7 +206,7 @@ int run_bwd(const FnetBlockNorm& a, hipStream_t st) {
         c.src[c.count] = s.plan.dst[i];
         c.dst[c.count] = out[i];
         c.groups[c.count] = by_sample ? s.plan.cut.samples : 1;
-        c.slots[c.count] = by_sample ? s.plan.cut.parts : i >= SUM_POST_W ? s.plan.cut.samples * s.plan.cut.parts : s.blocks;
+        c.slots[c.count] = by_sample ? s.plan.cut.parts : s.blocks;
         c.f32[c.count] = (i == SUM_GATE ? a.gate_dtype : a.param_dtype) == FNET_F32;
         groups += c.groups[c.count++];
     }

@@ -8,8 +8,7 @@ enum { SUM_PRE_W = 0, SUM_PRE_B, SUM_POST_W, SUM_POST_B, SUM_SCALE, SUM_GATE, SU
 struct BwdPlan {
     uint64_t dst[SUM_COUNT];     // where a block leaves a sum: its row of the partial sums, or (direct) the gradient itself; 0: nowhere
     int direct;                  // bit i: dst[i] is the gradient, in its own type
-    // the sums of the branch's side are left per segment (a sample's gate is part of them), those of the second norm per block; only with a
-    // gate per sample does a block go through several segments
+    // the gate's sums are left per segment, the others per block; only with a gate per sample does a block go through several segments
     RowCut cut;
     int in_turn;                 // a sample's rows are dealt to its parts in turn; otherwise each part is a run of rows
 };
@@ -159,8 +158,15 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
         if ((plan.direct >> which & 1) && !f32) gptr<T>(plan.dst[which])[to] = f_to_elem<T>(v);
         else gptr<float>(plan.dst[which])[to] = v;
     };
-    // the branch's sums, each times its factor (see above), to row `to` of their destinations: one column per thread
-    auto leave_branch_sums = [&](long long to, long long gate_at) {
+    // a sum of several segments: a sample's gate is part of each, so they are added up where the block leaves them (always the same thread's
+    // column).  A row of partial sums per segment instead: 262144 samples of 2 x 64 bf16 2165 us, now 1380; 65536 of 8 x 512 1273 and 996.
+    auto leave_more = [&](int which, bool more, int c, float v) {
+        if (more) v += gptr<const float>(plan.dst[which])[(long long)blockIdx.x * C + c];
+        leave(which, blockIdx.x, c, v, pf);
+    };
+    // the branch's sums over a segment, each times its factor (see above): one column per thread
+    auto leave_branch_sums = [&](int seg, long long gate_at) {
+        const bool more = seg != (int)blockIdx.x;
         if (!(plan.dst[SUM_POST_W] || plan.dst[SUM_POST_B] || plan.dst[SUM_SCALE] || plan.dst[SUM_GATE])) return;
         __syncthreads();
         collect(ao, W_O);
@@ -171,12 +177,12 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
             const float sc = a.residual_scale * (a.scale ? load_param1<T>(a.scale, c, pf) : 1.f);
             const float g = GM == GM_CONST && a.gate ? load_param1<T>(a.gate, gate_at + c, gf) : 0.f;
             const float f = GM == GM_CONST && a.gate ? gate_value(g, a.gate_act) : 1.f;
-            if (plan.dst[SUM_POST_W]) leave(SUM_POST_W, to, c, sc * f * p1, pf);
-            if (BIAS && plan.dst[SUM_POST_B]) leave(SUM_POST_B, to, c, sc * f * p0, pf);
+            if (plan.dst[SUM_POST_W]) leave_more(SUM_POST_W, more, c, sc * f * p1);
+            if (BIAS && plan.dst[SUM_POST_B]) leave_more(SUM_POST_B, more, c, sc * f * p0);
             if (plan.dst[SUM_SCALE] || plan.dst[SUM_GATE]) {
                 const float u = (a.post_weight ? load_param1<T>(a.post_weight, c, pf) : 1.f) * p1 + (BIAS && a.post_bias ? load_param1<T>(a.post_bias, c, pf) * p0 : 0.f);
-                if (plan.dst[SUM_SCALE]) leave(SUM_SCALE, to, c, a.residual_scale * f * u, pf);
-                if (plan.dst[SUM_GATE]) leave(SUM_GATE, to, c, sc * gate_slope(g, a.gate_act) * u, gf);
+                if (plan.dst[SUM_SCALE]) leave_more(SUM_SCALE, more, c, a.residual_scale * f * u);
+                if (plan.dst[SUM_GATE]) leave(SUM_GATE, seg, c, sc * gate_slope(g, a.gate_act) * u, gf);
             }
         }
     };

@@ -139,6 +139,14 @@ def test_many_rows(width, rows):
     both(t, dy, dh, act="tanh")
 
 
+@pytest.mark.parametrize("shape", [(2500, 2, 40), (3000, 2, 520), (1700, 3, 1300), (900, 2, 2309), (600, 2, 8200)], ids=str)
+def test_many_samples(shape):
+    """Several samples to a block, each with its gate: the sums over all of them, in every layout of rows."""
+    for kind, act, dtype, bias in (("layer", "sigmoid", BF16, True), ("rms", "tanh", F32, False)):
+        t, dy, dh = operands(shape, dtype, gate="sample", scale=True, bias=bias, seed=shape[2])
+        both(t, dy, dh, kind=kind, act=act)
+
+
 def test_no_second_derivative():
     t, dy, dh = operands((3, 16), F32)
     d = gpu(t, True)
