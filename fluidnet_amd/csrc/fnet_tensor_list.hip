@@ -531,7 +531,7 @@ int fnet_list_adam(int32_t n, const uint64_t* host_param, const uint64_t* host_g
     int rc = check_dense(n, host_param, host_numel, host_dtype);
     if (rc == FNET_OK) rc = check_dense(n, host_grad, host_numel, host_dtype);
     if (rc != FNET_OK) return rc;
-    FNET_CHECK_ARG(h->clock && (h->max_norm < 0.0 || (h->partials && h->n_partials >= 0)));
+    FNET_CHECK_ARG(h->clock && (h->max_norm < 0.0 || (h->partials && h->capacity >= 0)));
     FNET_CHECK_ARG(h->beta1 >= 0.0 && h->beta1 < 1.0 && h->beta2 >= 0.0 && h->beta2 < 1.0 && h->eps >= 0.0 && h->weight_decay >= 0.0);
     FNET_CHECK_ARG(std::isfinite(h->lr) && std::isfinite(h->weight_decay) && std::isfinite(h->eps) && !std::isnan(h->max_norm));
     for (int k = 0; k < n; ++k) {
@@ -539,7 +539,7 @@ int fnet_list_adam(int32_t n, const uint64_t* host_param, const uint64_t* host_g
         FNET_CHECK_ARG(host_exp_avg[k] && host_exp_avg_sq[k] && host_exp_avg[k] % 4 == 0 && host_exp_avg_sq[k] % 4 == 0);
         FNET_CHECK_ARG(host_dtype[k] == FNET_F32 || (host_master && host_master[k] && host_master[k] % 4 == 0));
     }
-    // everything that is written must lie apart (a gradient is only read)
+    // everything that is written must lie apart, and no gradient in it (gradients are only read: they may share memory among themselves)
     Span* spans = (Span*)malloc(sizeof(Span) * 4 * (size_t)n);
     if (!spans) return FNET_E_HIP;
     int m = 0;
@@ -552,10 +552,22 @@ int fnet_list_adam(int32_t n, const uint64_t* host_param, const uint64_t* host_g
         if (host_dtype[k] != FNET_F32) spans[m++] = Span{host_master[k], host_master[k] + bytes};
     }
     rc = apart(spans, m);
+    for (int k = 0; k < n && rc == FNET_OK; ++k) {
+        const uint64_t lo = host_grad[k], hi = lo + (uint64_t)host_numel[k] * elem_size(host_dtype[k]);
+        const Span* next = std::lower_bound(spans, spans + m, hi, [](const Span& s, uint64_t end) { return s.lo < end; });
+        if (hi > lo && next != spans && next[-1].hi > lo) rc = FNET_E_OVERLAP;
+    }
     free(spans);
     if (rc != FNET_OK) return rc;
+    // the clock moves with the first launch, so everything that can be refused has been by now
+    int32_t used = 0;
+    rc = h->max_norm < 0.0 ? fnet_list_clock(h->clock, h->beta1, h->beta2, stream)
+                           : fnet_list_norm_partials(n, host_grad, host_numel, host_dtype, 0, nullptr, NORM_2, h->partials, h->capacity, &used,
+                                                     h->clock, h->beta1, h->beta2, stream);
+    if (rc != FNET_OK) return rc;
+    if (used == 0 && h->max_norm >= 0.0 && h->norm_out) return fnet_list_norm_finish(h->partials, 0, NORM_2, h->norm_out, stream);   // no elements at all
     AdamArgs a{};
-    a.f = ClipFrom{h->partials, nullptr, h->n_partials, NORM_2, h->max_norm, h->norm_out};
+    a.f = ClipFrom{h->partials, nullptr, used, NORM_2, h->max_norm, h->norm_out};
     a.clip = h->max_norm >= 0.0;
     a.clock = h->clock;
     a.lr_dev = h->lr_device;

@@ -94,11 +94,15 @@ class TensorList:
     def args(self):
         return self.n, self.ptrs, self.numels, self.codes, self.n_strided, self.strided
 
-    def partials(self, kind: int, clock: int = 0, beta1: float = 0.0, beta2: float = 0.0):
+    def workspace(self) -> torch.Tensor:
+        """Room for the partial sums of the norm."""
+        return torch.empty(self.capacity, dtype=torch.float64, device=self.first.device)
+
+    def partials(self, kind: int):
         """(workspace, how many partial sums are in it)."""
-        ws = torch.empty(self.capacity, dtype=torch.float64, device=self.first.device)
+        ws = self.workspace()
         used = ctypes.c_int32()
-        rt.call_on(self.first, "fnet_list_norm_partials", *self.args(), kind, ws.data_ptr(), self.capacity, ctypes.byref(used), clock, beta1, beta2)
+        rt.call_on(self.first, "fnet_list_norm_partials", *self.args(), kind, ws.data_ptr(), self.capacity, ctypes.byref(used), 0, 0.0, 0.0)
         return ws, used.value
 
     def norm(self, kind: int) -> torch.Tensor:

@@ -116,7 +116,8 @@ def clip_adam_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     The gradients are not changed: the clipped ones are never written.  Returns the norm before clipping (0-dim, fp32, on the device; None
     without clipping).  params[k] and grads[k] are of one type (fp32, bf16 or fp16); exp_avgs and exp_avg_sqs are fp32; all of them are dense and
     laid out alike.  Parameters that are not fp32 need an fp32 master each: the master is updated and the parameter is its rounding (masters
-    of fp32 parameters are not looked at).  Parameters, moments and masters that share memory are refused.  clock: three fp64 values on the device, t, beta1^t and beta2^t of the steps done so far; the call advances it.  lr: a number,
+    of fp32 parameters are not looked at).  Parameters, moments and masters that share memory, with each other or with a gradient, are
+    refused.  clock: three fp64 values on the device, t, beta1^t and beta2^t of the steps done so far; the call advances it.  lr: a number,
     or one fp64 value on the device, which a captured step reads anew at every replay.  Two launches for up to 80 parameters."""
     params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
     n = len(params)
@@ -149,17 +150,13 @@ def clip_adam_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         for k in low:
             ptrs[3][k] = masters[k].data_ptr()
     address = [a.buffer_info()[0] for a in ptrs] + [None] * (4 - len(ptrs))
-    total, partials, used = None, None, 0
+    total, ws = None, None
     if max_norm is not None:
         total = torch.empty((), dtype=f32, device=lst.first.device)
-        partials, used = lst.partials(0, clock.data_ptr(), b1, b2)
-        if used == 0:
-            total.zero_()                       # only parameters of no elements
-    else:
-        rt.call_on(lst.first, "fnet_list_clock", clock.data_ptr(), b1, b2)
+        ws = lst.workspace()
     a = _ADAM.pack(0.0 if isinstance(lr, torch.Tensor) else float(lr), b1, b2, eps, weight_decay, -1.0 if max_norm is None else max_norm,
-                   0 if partials is None else partials.data_ptr(), clock.data_ptr(), lr.data_ptr() if isinstance(lr, torch.Tensor) else 0,
-                   0 if total is None else total.data_ptr(), used)
+                   0 if ws is None else ws.data_ptr(), clock.data_ptr(), lr.data_ptr() if isinstance(lr, torch.Tensor) else 0,
+                   0 if total is None else total.data_ptr(), 0 if ws is None else lst.capacity)
     rt.call_on(lst.first, "fnet_list_adam", n, address[0], lst.ptrs, address[1], address[2], address[3], lst.numels, lst.codes, a)
     torch.autograd.graph.increment_version(params)
     return total

@@ -320,11 +320,12 @@ int fnet_block_norm_workspace(const FnetBlockNorm* host_args, int64_t* bytes);
  * tensor of any layout is its memory in order.  Entries of no elements are skipped.  All of it is capturable.
  *   fnet_list_norm_partials  sums of squares / of absolutes / maxima of the list's parts in 64 bits, *n_partials of them (at most `capacity`,
  *                            which 2048 + n / 64 + 256 * n_strided + 8 always covers); `clock`, if not 0, is advanced as one Adam step
- *   fnet_list_clock          advances clock = (t, beta1^t, beta2^t) alone (a step without clipping)
+ *   fnet_list_clock          advances clock = (t, beta1^t, beta2^t) alone
  *   fnet_list_norm_finish    the norm itself from the partials
  *   fnet_list_scale          g *= min(1, max_norm / (norm + 1e-6)), the norm taken from the partials, or from *norm if those are 0; the
  *                            norm is also stored to *norm_out if that is not 0.  FNET_E_OVERLAP if two dense tensors share memory
- *   fnet_list_adam           one step; parameters that are not fp32 have an fp32 master that is updated and of which they are the rounding
+ *   fnet_list_adam           one whole step: norm, clock, update.  Parameters that are not fp32 have an fp32 master that is updated and of
+ *                            which they are the rounding.  FNET_E_OVERLAP if what is written shares memory, with itself or with a gradient
  */
 #define FNET_LIST_MAXDIM 6
 #define FNET_LIST_NORM_2 0
@@ -338,11 +339,11 @@ typedef struct FnetStridedTensor {    /* a tensor that is no dense block: sizes 
 typedef struct FnetAdamList {
     double lr, beta1, beta2, eps, weight_decay;
     double max_norm;          /* < 0: no clipping */
-    const double* partials;   /* device: from fnet_list_norm_partials over the gradients (2-norm) */
-    const double* clock;      /* device: t, beta1^t, beta2^t of this step (already advanced) */
+    double* partials;         /* device, for clipping: `capacity` values of workspace, as in fnet_list_norm_partials */
+    double* clock;            /* device: t, beta1^t, beta2^t of the steps done so far; advanced */
     const double* lr_device;  /* device, or 0: lr */
-    float* norm_out;          /* device, or 0: the norm before clipping */
-    int32_t n_partials;
+    float* norm_out;          /* device, or 0: the 2-norm of the gradients before clipping */
+    int32_t capacity;
 } FnetAdamList;
 int fnet_list_norm_partials(int32_t n, const uint64_t* host_ptr, const int64_t* host_numel, const int32_t* host_dtype, int32_t n_strided,
                             const FnetStridedTensor* host_strided, int32_t norm_kind, double* partials, int32_t capacity,

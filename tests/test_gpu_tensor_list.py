@@ -269,6 +269,20 @@ def test_adam_refusals():
         clip_adam_([p[0], p[0]], g, m, v, clock, masters=w, **kw)
 
 
+def test_refused_step_changes_nothing():
+    """A step that is refused for what it would write leaves the clock as it was, too; gradients may share memory among themselves only."""
+    p, g, m, v, w = _state([8, 8, 0], F32)
+    clock = torch.tensor([3.0, 0.9 ** 3, 0.999 ** 3], dtype=torch.float64, device="cuda")
+    before = [t.clone() for t in (*p, *g, *m, *v, clock)]
+    for args in (([p[0], p[0], p[2]], g, m, v), (p, [m[1], g[1], g[2]], m, v), (p, [g[0], p[0], g[2]], m, v), (p, g, m, m)):
+        for max_norm in (1.0, None):
+            with pytest.raises(FluidNetHipError, match="share memory"):
+                clip_adam_(*args, clock, lr=1e-3, max_norm=max_norm)
+    assert all(torch.equal(a, b) for a, b in zip(before, (*p, *g, *m, *v, clock)))
+    clip_adam_(p, [g[0], g[0], g[2]], m, v, clock, lr=1e-3, max_norm=1.0)
+    assert clock[0].item() == 4.0 and not torch.equal(m[0], before[6])
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
 def test_optimizer_against_torch(dtype):
     """Ten steps of ClipAdam and of torch's clip_grad_norm_ + AdamW in 64 bits on the same gradients.  Each step adds at most the bound of one

@@ -111,3 +111,7 @@ def test_c_adam_refuses():
         assert adam(**over) == -1, over
     for over in (dict(p=(0x1000, 0x1010)), dict(m=(0x5000, 0x5000)), dict(v=(0x5004, 0x8000)), dict(dtype=(1, 1), w=(0x1000, 0x9000))):
         assert adam(**over) == -5, over
+    # a gradient is read while other blocks write, so it may lie in nothing that is written
+    for over in (dict(g=(0x5000, 0x4000)), dict(g=(0x3000, 0x1ffc)), dict(g=(0x101c, 0x4000), most=-1.0), dict(g=(0x701c, 0x4000)),
+                 dict(dtype=(1, 1), w=(0xa000, 0x9000), g=(0x901e, 0x4000))):
+        assert adam(**over) == -5, over
