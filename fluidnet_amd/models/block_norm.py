@@ -20,11 +20,17 @@ spaced, or the operand is copied first; slices of the last axis are taken as the
 all in x's type.  gate, in fp32 or x's type: like x (a value per element), [..., 1] (per token), [B, 1, .., 1, C] for x [B, .., C] (per sample)
 or [C] (per channel); gate_act "identity", "sigmoid" or "tanh".  A NaN or infinity stays in its row (and in the sums over rows).
 There is no CPU fallback, and no second derivative (asking for one raises).
+
+Both directions can be captured into a graph.  A captured backward pass that hands gradients to leaves (into .grad or out of
+torch.autograd.grad) raises while outputs of an eager call from the same leaves on the default stream are alive: torch orders a leaf's gradient
+after the stream on which the leaf was first used, the default stream cannot take part in a capture, and the process would end.  Drop those
+outputs first, or make the eager calls on a side stream.  (Outputs of other operations on the same leaves are the caller's to drop.)
 """
 from __future__ import annotations
 
 import ctypes
 import struct
+import weakref
 from typing import Literal, Optional, Tuple
 
 import torch
@@ -259,17 +265,55 @@ def _backward(ctx, dy, dh):
 _backward_once = once_differentiable(_backward)
 
 
+_on_default = weakref.WeakSet()              # nodes of the graphs that are alive and were made on the default stream
+
+
+def _leaf_nodes(node) -> dict:
+    """The nodes of leaves in the graph below `node`, by the leaf's identity."""
+    seen, todo, leaves = {node}, [node], {}
+    while todo:
+        for below, _ in todo.pop().next_functions:
+            if below is not None and below not in seen:
+                seen.add(below)
+                todo.append(below)
+                if hasattr(below, "variable"):
+                    leaves[id(below.variable)] = below
+    return leaves
+
+
+def _wanted(node) -> bool:
+    try:
+        return torch._C._will_engine_execute_node(node)
+    except RuntimeError:                      # torch.autograd.grad is asked for this leaf's
+        return True
+
+
+def _check_capture(ctx) -> None:
+    """While a graph is captured: raises if a leaf's gradient would be ordered after the default stream (see above)."""
+    eager = [node for node in (ref() for ref in list(_on_default.data)) if node is not None]
+    if not eager:
+        return
+    mine = {leaf for leaf, node in _leaf_nodes(ctx).items() if _wanted(node)}
+    if mine and any(mine & _leaf_nodes(node).keys() for node in eager):
+        raise RuntimeError("outputs of an earlier call from the same leaves, made on the default stream, are alive: drop them before capturing "
+                           "a backward pass")
+
+
 class _BlockNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, s, x, branch, gate, scale, pw, pb, nw, nb):
         ctx.set_materialize_grads(False)
         y, h, stats = _forward(s, x, branch, gate, scale, pw, pb, nw, nb, True)
         ctx.s = s
+        if rt.raw_stream(x.get_device()) == 0:
+            _on_default.add(ctx)
         ctx.save_for_backward(x, branch, gate, scale, pw, pb, nw, nb, stats)
         return y, h
 
     @staticmethod
     def backward(ctx, dy, dh):
+        if torch.cuda.is_current_stream_capturing():
+            _check_capture(ctx)
         # with create_graph the gradients are marked as having no derivative of their own; without it nobody can ask for one
         return _backward_once(ctx, dy, dh) if torch.is_grad_enabled() else _backward(ctx, dy, dh)
 

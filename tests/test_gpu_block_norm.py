@@ -1,5 +1,6 @@
 """The norms around a residual block (fluidnet_amd/models/block_norm.py) against their definition in 64 bits: types, widths from 1 to the
 largest of every row layout, gates of every shape, strides, no rows, values that are not finite, other streams, graphs."""
+import gc
 import itertools
 
 import pytest
@@ -362,6 +363,53 @@ def test_graph_forward_and_backward():
         torch.cuda.synchronize()
         want = once(gpu(new, True))
         assert all(torch.equal(p, q) for p, q in zip(out, want)), seed
+
+
+@pytest.mark.parametrize("through", [False, True], ids=["leaf", "view"])
+def test_captured_backward_next_to_an_eager_graph(through):
+    """A captured backward pass of leaves whose eager graph on the default stream is alive is refused before torch hands anything to a leaf; with
+    that graph dropped, or made on a side stream, it is captured and accumulates at every replay."""
+    w = torch.rand(264, device="cuda").requires_grad_()
+    b = torch.rand(264, device="cuda").requires_grad_()
+    x = torch.randn(40, 264, device="cuda")
+    up = torch.ones(40, 264, device="cuda")
+    param = (lambda: (w[:], b[:])) if through else (lambda: (w, b))
+
+    def once():
+        pw, pb = param()
+        return gated_residual(x, x, post_weight=pw, pre_weight=pb)[1]
+    eager = once()
+    eager.backward(up)
+    want, w.grad, b.grad = (w.grad, b.grad), torch.zeros_like(w), torch.zeros_like(b)
+    for t in (w, b):
+        torch.autograd.graph.get_gradient_edge(t).node.metadata["eager"] = True
+    torch.cuda.synchronize()
+    for backward in (lambda h: h.backward(up), lambda h: torch.autograd.grad(h, [w, b], up), lambda h: torch.autograd.grad(h, [b], up)):
+        with pytest.raises(RuntimeError, match="are alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                backward(once())
+        torch.cuda.synchronize()
+    assert not w.grad.any() and not b.grad.any()
+    del eager
+    gc.collect()
+    # the leaves' nodes are new ones: nothing of the eager graph is left that the capture below could meet
+    assert not any(torch.autograd.graph.get_gradient_edge(t).node.metadata for t in (w, b))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        once().backward(up)
+    torch.cuda.current_stream().wait_stream(side)
+    w.grad.zero_()
+    b.grad.zero_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        once().backward(up)
+    for k in (1, 2, 3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, g in zip((w, b), want):
+            # k equal terms added up in fp32: each addition is off by half a step at most
+            assert ((a.grad.double() - k * g.double()).abs() <= k * 2.0 ** -23 * k * g.double().abs()).all(), k
 
 
 def test_large_offsets():
