@@ -1,8 +1,9 @@
-"""Build libfluidnet_hip.so in-tree with hipcc for gfx950 (cross-compiles without a GPU).
+"""Build libfluidnet_hip.so in-tree with hipcc for gfx950 (cross-compiles without a GPU), and engine/_torch_ops.so, the host side of the
+operators on torch tensors, with the host compiler against torch's headers.
 
     python -m fluidnet_amd.build [--force]
 
-The .so lands in fluidnet_amd/lib/ (git-ignored, but it travels to the GPU box with the tree).
+Both are git-ignored.
 """
 from __future__ import annotations
 
@@ -24,6 +25,10 @@ HEADERS = [os.path.join(CSRC, h) for h in ("fnet_common.h", "fnet_vec.h", "fnet_
 # MI355X now and then; the scalar forms are as fast for code that memory bounds.  (The host pass warns that it does not know the feature.)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-ffp-contract=off", "-Wall", "-Wno-unused-function", "-Wno-unused-value",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
+CXX = os.environ.get("CXX", "g++")
+TORCH_OPS_SRC = os.path.join(CSRC, "torch_ops.cpp")
+TORCH_OPS = os.path.join(HERE, "engine", "_torch_ops.so")
 
 
 def _hipcc() -> str:
@@ -51,13 +56,16 @@ def build(force: bool = False, verbose: bool = True) -> str:
         objs.append(obj)
         if force or _stale(obj, [src] + HEADERS):
             jobs.append([hipcc, *FLAGS, "-c", src, "-o", obj])
+    ops_obj = os.path.join(LIBDIR, "torch_ops.o")
+    if force or _stale(ops_obj, [TORCH_OPS_SRC, HEADERS[-1]]):
+        jobs.append([CXX, *_torch_flags(), "-c", TORCH_OPS_SRC, "-o", ops_obj])
 
     def run(cmd):
         if verbose:
             print(" ".join(cmd), flush=True)
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
-            raise RuntimeError(f"hipcc failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+            raise RuntimeError(f"build failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
         if verbose and r.stderr.strip():
             print(r.stderr, file=sys.stderr)
 
@@ -66,7 +74,26 @@ def build(force: bool = False, verbose: bool = True) -> str:
     if force or jobs or _stale(LIB, objs):
         # -z defs: an unresolved kernel stub must fail the build here, not the dlopen on the GPU box
         run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-Wl,-z,defs", "-o", LIB, *objs])
+    if force or jobs or _stale(TORCH_OPS, [ops_obj, LIB]):
+        at = _torch_dir()
+        run([CXX, "-shared", "-o", TORCH_OPS, ops_obj, f"-L{at}/lib", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip", "-lamdhip64",
+             f"-L{LIBDIR}", "-lfluidnet_hip", "-Wl,-rpath,$ORIGIN/../lib"])
     return LIB
+
+
+def _torch_dir() -> str:
+    import torch
+    return os.path.dirname(torch.__file__)
+
+
+def _torch_flags():
+    import sysconfig
+
+    import torch
+    at = _torch_dir()
+    include = (f"{at}/include", f"{at}/include/torch/csrc/api/include", sysconfig.get_path("include"), os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include"))
+    return ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-isystem{i}" for i in include)]
 
 
 if __name__ == "__main__":

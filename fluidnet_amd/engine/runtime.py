@@ -114,6 +114,24 @@ def lib() -> ctypes.CDLL:
     return L
 
 
+_torch_ops = None
+
+
+def torch_ops():
+    """The native host side of the operators on torch tensors (csrc/torch_ops.cpp; built by `python -m fluidnet_amd.build`)."""
+    global _torch_ops
+    if _torch_ops is None:
+        import torch  # noqa: F401  (its libraries have to be there first)
+        lib()
+        try:
+            from . import _torch_ops as ops
+        except ImportError as e:
+            raise FluidNetHipError(f"fluidnet_amd/engine/_torch_ops.so does not load ({e}): build it with `python -m fluidnet_amd.build`") from e
+        ops.set_error(FluidNetHipError)
+        _torch_ops = ops
+    return _torch_ops
+
+
 EXPORTS = ["fnet_abi_version", "fnet_strerror", "fnet_last_hip_error", "fnet_device_info", "fnet_plan_run", "fnet_lane_stream", "fnet_set_knob", "fnet_physics_loss_terms_noalloc", "fnet_graph_create",
            "fnet_graph_launch", "fnet_graph_destroy", "fnet_spatial_gradients", "fnet_divergence", "fnet_timer_create",
            "fnet_timer_start", "fnet_timer_stop", "fnet_timer_elapsed_ms", "fnet_timer_destroy", "fnet_unet_param_count",

@@ -13,8 +13,6 @@ from __future__ import annotations
 import ctypes
 import math
 import struct
-from array import array
-from operator import attrgetter
 from typing import Iterable, List, Union
 
 import torch
@@ -45,37 +43,34 @@ def _collapsed(t: torch.Tensor):
     return out
 
 
-# Over hundreds of tensors the checks cost more than the kernels: each is one pass of C code over the list, and only a list that fails one is
-# looked at tensor by tensor.
-_device, _contiguous, _numel, _address = (getattr(torch.Tensor, n) for n in ("get_device", "is_contiguous", "numel", "data_ptr"))
-_dtype, _shape = attrgetter("dtype"), attrgetter("shape")
-
-
 class TensorList:
     """Addresses, element counts and types of the tensors of a call, as the C ABI takes them.  Lives for the call only."""
 
     def __init__(self, tensors: List[torch.Tensor], what: str = "gradient") -> None:
         self.first = tensors[0]
-        device = self.first.get_device()
-        if device < 0:
-            raise RuntimeError(f"fluidnet_amd runs on MI355X only (got a CPU {what}); there is no CPU fallback")
-        types = list(map(_dtype, tensors))
-        if not (ELEM.keys() >= set(types) and set(map(_device, tensors)) == {device}):
-            k, t = next((k, t) for k, t in enumerate(tensors) if t.dtype not in ELEM or t.get_device() != device)
-            raise ValueError(f"{what} {k} must be a float32, bfloat16 or float16 tensor on {self.first.device} (got {t.dtype} on {t.device})")
+        table = rt.torch_ops().tensor_table(tensors)
+        if table is None:
+            self._refuse(tensors, what)
         strided = []
-        self.contiguous = all(map(_contiguous, tensors))
-        if not self.contiguous:
-            tensors, types, strided = self._split(tensors, what)
-        self.n, self.n_strided, self.types = len(tensors), len(strided), types
-        self._keep = (array("Q", map(_address, tensors)), array("q", map(_numel, tensors)), array("i", map(ELEM.__getitem__, types)), b"".join(strided))
-        self.ptrs, self.numels, self.codes = (a.buffer_info()[0] for a in self._keep[:3])
-        self.strided = ctypes.cast(ctypes.c_char_p(self._keep[3]), ctypes.c_void_p) if strided else None
+        if not table[0]:
+            tensors, strided = self._split(tensors, what)
+            table = rt.torch_ops().tensor_table(tensors)
+        self.n, self.n_strided = len(tensors), len(strided)
+        _, self.ptrs, self.numels, self.codes = table           # as bytes
+        self.strided = b"".join(strided) if strided else None
         self.capacity = 2048 + self.n // 64 + 256 * self.n_strided + 8
 
     @staticmethod
+    def _refuse(tensors, what):
+        first = tensors[0]
+        if not first.is_cuda:
+            raise RuntimeError(f"fluidnet_amd runs on MI355X only (got a CPU {what}); there is no CPU fallback")
+        k, t = next((k, t) for k, t in enumerate(tensors) if t.dtype not in ELEM or t.device != first.device or t.is_neg())
+        raise ValueError(f"{what} {k} must be a float32, bfloat16 or float16 tensor on {first.device} and no negated view (got {t.dtype} on {t.device})")
+
+    @staticmethod
     def _split(tensors, what):
-        """The dense tensors, their types, and the records of those that are no dense block of memory."""
+        """The dense tensors, and the records of those that are no dense block of memory."""
         dense, strided = [], []
         for k, t in enumerate(tensors):
             axes = [[1, t.numel()]] if t.is_contiguous() else _collapsed(t)
@@ -89,7 +84,7 @@ class TensorList:
                 dense.append(t)
         if len(set(strided)) != len(strided):
             raise ValueError(f"a {what} appears twice")
-        return dense, [t.dtype for t in dense], strided
+        return dense, strided
 
     def args(self):
         return self.n, self.ptrs, self.numels, self.codes, self.n_strided, self.strided

@@ -9,7 +9,6 @@ from __future__ import annotations
 
 import math
 import struct
-from array import array
 from typing import Dict, Iterable, List, Optional, Sequence, Union
 
 import numpy as np
@@ -17,7 +16,7 @@ import torch
 
 from ..engine import runtime as rt
 from ..engine.runtime import OPC
-from .grad_clip import TensorList, _address, _collapsed, _contiguous, _device, _dtype, _max_norm, _numel, _shape
+from .grad_clip import TensorList, _collapsed, _max_norm
 
 
 class FusedClipAdam:
@@ -82,7 +81,7 @@ class FusedClipAdam:
 # ---------------------------------------------------------------------------------------------------------------- lists of parameters
 def _same_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two tensors are dense and element k of one lies where element k of the other does."""
-    if a.shape != b.shape:
+    if a.shape != b.shape or a.is_neg() or b.is_neg():
         return False
     if a.is_contiguous() and b.is_contiguous():
         return True
@@ -96,6 +95,8 @@ _ADAM = struct.Struct("=6d4Qi4x")
 def _check_layouts(params, grads, exp_avgs, exp_avg_sqs, masters) -> None:
     """Tensor by tensor what clip_adam_ asks of a whole list: raises for the first one that does not fit; dense tensors in another order pass."""
     for k, (p, g, m, v, w) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs, masters)):
+        if w is None and p.dtype is not torch.float32:
+            raise ValueError(f"parameter {k} is not float32 and needs an fp32 master")
         if p.dtype is not g.dtype or p.get_device() != g.get_device() or not _same_layout(p, g):
             raise ValueError(f"parameter {k} and its gradient must be dense tensors of one type, layout and device (got "
                              f"{tuple(p.shape)} {p.stride()} {p.dtype} {p.device}, {tuple(g.shape)} {g.stride()} {g.dtype} {g.device})")
@@ -129,30 +130,17 @@ def clip_adam_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         raise ValueError(f"betas must lie in [0, 1), eps and weight_decay must not be negative (got {betas}, {eps}, {weight_decay})")
     if max_norm is not None:
         max_norm = _max_norm(max_norm)
-    lst = TensorList(grads)
-    dev, f32 = lst.first.get_device(), torch.float32
-    types = list(map(_dtype, params))
-    low = [k for k, t in enumerate(types) if t is not f32]
-    if any(masters[k] is None for k in low):
-        raise ValueError(f"parameter {next(k for k in low if masters[k] is None)} is not float32 and needs an fp32 master")
-    state = exp_avgs + exp_avg_sqs + [masters[k] for k in low]
-    numels = list(map(_numel, params))
-    if not (lst.contiguous and types == lst.types and set(map(_dtype, state)) == {f32} and set(map(_device, params + state)) == {dev}
-            and list(map(_shape, params)) == list(map(_shape, grads)) and list(map(_numel, state)) == numels + numels + [numels[k] for k in low]
-            and all(map(_contiguous, params + state))):
+    lst, ops = TensorList(grads), rt.torch_ops()
+    if not ops.adam_fits(params, grads, exp_avgs, exp_avg_sqs, masters):
         _check_layouts(params, grads, exp_avgs, exp_avg_sqs, masters)
+    dev = lst.first.get_device()
     for name, t, count in (("clock", clock, 3),) + ((("lr", lr, 1),) if isinstance(lr, torch.Tensor) else ()):
         if t.dtype is not torch.float64 or t.numel() != count or t.get_device() != dev or not t.is_contiguous():
             raise ValueError(f"{name} must be {count} float64 value(s) on {lst.first.device}")
-    ptrs = [array("Q", map(_address, ts)) for ts in (params, exp_avgs, exp_avg_sqs)]
-    if low:
-        ptrs.append(array("Q", [0] * n))
-        for k in low:
-            ptrs[3][k] = masters[k].data_ptr()
-    address = [a.buffer_info()[0] for a in ptrs] + [None] * (4 - len(ptrs))
+    address = [ops.addresses(ts) for ts in (params, exp_avgs, exp_avg_sqs, masters)]
     total, ws = None, None
     if max_norm is not None:
-        total = torch.empty((), dtype=f32, device=lst.first.device)
+        total = torch.empty((), dtype=torch.float32, device=lst.first.device)
         ws = lst.workspace()
     a = _ADAM.pack(0.0 if isinstance(lr, torch.Tensor) else float(lr), b1, b2, eps, weight_decay, -1.0 if max_norm is None else max_norm,
                    0 if ws is None else ws.data_ptr(), clock.data_ptr(), lr.data_ptr() if isinstance(lr, torch.Tensor) else 0,
@@ -203,7 +191,7 @@ class ClipAdam:
         self._clock = torch.tensor([0.0, 1.0, 1.0], dtype=torch.float64, device=dev)
         self._lr = torch.tensor(self.param_groups[0]["lr"], dtype=torch.float64, device=dev)
         self._lr_pushed = self.param_groups[0]["lr"]
-        self._seen = [(p.data_ptr(), p._version) for p in self.params]
+        self._seen = rt.torch_ops().marks(self.params)
         if old is not None:
             self.load_state_dict(old)
 
@@ -214,7 +202,7 @@ class ClipAdam:
         for w, p in zip(self._w, self.params):
             if w is not None:
                 w.copy_(p)
-        self._seen = [(p.data_ptr(), p._version) for p in self.params]
+        self._seen = rt.torch_ops().marks(self.params)
 
     def push_lr(self) -> None:
         """Copies param_groups[0]["lr"] to the device, where a captured step reads it."""
@@ -236,11 +224,13 @@ class ClipAdam:
     def step(self) -> None:
         self._init_state()
         self.push_lr()
-        for k, (p, w, seen) in enumerate(zip(self.params, self._w, self._seen)):
-            if w is not None and seen != (p.data_ptr(), p._version):
-                if torch.cuda.is_current_stream_capturing():
-                    raise RuntimeError("ClipAdam: a parameter was written since the last step; call refresh() before capturing the step")
-                w.copy_(p)
+        marks = rt.torch_ops().marks(self.params)
+        if marks != self._seen:
+            for k, (p, w) in enumerate(zip(self.params, self._w)):
+                if w is not None and marks[16 * k:16 * k + 16] != self._seen[16 * k:16 * k + 16]:
+                    if torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("ClipAdam: a parameter was written since the last step; call refresh() before capturing the step")
+                    w.copy_(p)
         have = [k for k, p in enumerate(self.params) if p.grad is not None]
         if not have:
             return
@@ -249,7 +239,7 @@ class ClipAdam:
         grads = [p.grad if _same_layout(p, p.grad) else torch.empty_like(p).copy_(p.grad) for p in params]
         self.grad_norm = clip_adam_(params, grads, pick(self._m), pick(self._v), self._clock, masters=pick(self._w), lr=self._lr, betas=self.betas,
                                     eps=self.eps, weight_decay=self.weight_decay, max_norm=self.max_norm)
-        self._seen = [(p.data_ptr(), p._version) for p in self.params]
+        self._seen = rt.torch_ops().marks(self.params)
 
     @property
     def step_count(self) -> int:
@@ -277,4 +267,4 @@ class ClipAdam:
             if w is not None:
                 # a master that does not round to its parameter is not this parameter's (the model was loaded from elsewhere)
                 w.copy_(p if b is None else torch.where(b.to(w.device).to(p.dtype) == p, b.to(w.device), p.float()))
-        self._seen = [(p.data_ptr(), p._version) for p in self.params]
+        self._seen = rt.torch_ops().marks(self.params)

@@ -1,13 +1,15 @@
 """Refusals of the norms around a residual block, in Python and at the C entry points; none of them reaches the GPU."""
 import ctypes
+import struct
 
 import pytest
 import torch
 
 from fluidnet_amd.engine import runtime as rt
-from fluidnet_amd.models.block_norm import _ARGS, gated_residual, pre_norm
+from fluidnet_amd.models.block_norm import gated_residual, pre_norm
 
 X = torch.zeros(2, 3, 8)
+_ARGS = struct.Struct("=7q8i2f22Qq")             # struct FnetBlockNorm (include/fluidnet_hip.h)
 
 
 @pytest.mark.parametrize("match,call", [
