@@ -13,14 +13,15 @@ constexpr int kThreads = 256;
 // Every launch carries its part of the list as a kernel argument (below 4 KB): nothing is uploaded, so there is no table whose lifetime a
 // captured graph or another stream could outlive.
 constexpr int kTab = 240, kAdamTab = 96, kMasterTab = 80;
-constexpr long long kMaxEntry = 1ll << 30;       // a longer tensor takes several entries
+constexpr long long kMaxEntry = 1ll << 29;       // a longer tensor takes several entries
 constexpr int kMaxBlocks = 2048;                 // eight blocks of four waves per CU; also the number of partial sums every consumer re-reads
 
+constexpr uint32_t kCount = (1u << 30) - 1;
 enum { NORM_2 = 0, NORM_1 = 1, NORM_INF = 2 };
 
 struct ListTab {
     uint64_t p[kTab];
-    uint32_t n[kTab];            // elements
+    uint32_t n[kTab];            // elements, and the type from bit 30 on
     uint32_t first[kTab];        // index of the entry's first chunk in this launch
     int count;
     uint32_t chunks;
@@ -100,37 +101,51 @@ __device__ __forceinline__ void advance_clock(double* clock, double b1, double b
 constexpr int kNormVecs = 8;                      // 16-byte loads per lane and chunk
 template <typename T> __host__ __device__ constexpr uint32_t norm_chunk() { return (uint32_t)kThreads * VecOf<T>::V * kNormVecs; }
 
-template <typename T, int KIND>
+// f(T()); with T = void for the type of an entry, which is the same for the whole block.  A list of several types goes through kernels of that
+// kind, all types in one launch (41 tensors of three types: 27 us with a launch per type, 20 so); a list of one type through its own, which
+// are faster (403 M bf16: 395 us and 437).
+template <typename T, typename F>
+__device__ __forceinline__ void of_type(uint32_t n_and_type, F f) {
+    if constexpr (!std::is_void<T>::value) f(T());
+    else if (n_and_type >> 30 == FNET_F32) f(float());
+    else if (n_and_type >> 30 == FNET_BF16) f(bf16_t());
+    else f(f16_t());
+}
+
+template <typename LIST, int KIND>
 __global__ __launch_bounds__(256) void k_list_norm(ListTab t, double* partials, double* clock, double b1, double b2) {
-    constexpr int V = VecOf<T>::V;
     __shared__ double red[4];
     if (clock && blockIdx.x == 0 && threadIdx.x == 0) advance_clock(clock, b1, b2);
     double acc[4] = {0.0, 0.0, 0.0, 0.0};
     uint32_t mx = 0;
     for (uint32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
         const int j = find_entry(t, c);
-        const uint32_t n = t.n[j], at = (c - t.first[j]) * norm_chunk<T>();
-        const T* p = gptr<const T>(t.p[j]) + at;
-        const uint32_t left = n - at;
-        if (left >= norm_chunk<T>()) {
-            u32x4 w[kNormVecs];
+        of_type<LIST>(t.n[j], [&](auto type) {
+            using T = decltype(type);
+            constexpr int V = VecOf<T>::V;
+            const uint32_t n = t.n[j] & kCount, at = (c - t.first[j]) * norm_chunk<T>();
+            const T* p = gptr<const T>(t.p[j]) + at;
+            const uint32_t left = n - at;
+            if (left >= norm_chunk<T>()) {
+                u32x4 w[kNormVecs];
 #pragma unroll
-            for (int k = 0; k < kNormVecs; ++k) w[k] = *reinterpret_cast<const typename VecOf<T>::vec*>(p + (k * kThreads + threadIdx.x) * V);
+                for (int k = 0; k < kNormVecs; ++k) w[k] = *reinterpret_cast<const typename VecOf<T>::vec*>(p + (k * kThreads + threadIdx.x) * V);
 #pragma unroll
-            for (int k = 0; k < kNormVecs; ++k) {
-                float v[V];
-                unpack16<T>(w[k], v);
+                for (int k = 0; k < kNormVecs; ++k) {
+                    float v[V];
+                    unpack16<T>(w[k], v);
 #pragma unroll
-                for (int i = 0; i < V; ++i) norm_add<KIND>(acc[i & 3], mx, v[i]);
+                    for (int i = 0; i < V; ++i) norm_add<KIND>(acc[i & 3], mx, v[i]);
+                }
+            } else {
+                for (uint32_t o = threadIdx.x * V; o < left; o += kThreads * V) {
+                    float v[V];
+                    load_chunk<T>(p + o, (int)min(left - o, (uint32_t)V), v);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) norm_add<KIND>(acc[i & 3], mx, v[i]);
+                }
             }
-        } else {
-            for (uint32_t o = threadIdx.x * V; o < left; o += kThreads * V) {
-                float v[V];
-                load_chunk<T>(p + o, (int)min(left - o, (uint32_t)V), v);
-#pragma unroll
-                for (int i = 0; i < V; ++i) norm_add<KIND>(acc[i & 3], mx, v[i]);
-            }
-        }
+        });
     }
     const double mine = KIND == NORM_INF ? (double)__uint_as_float(mx) : (acc[0] + acc[1]) + (acc[2] + acc[3]);
     const double s = block_join<KIND>(mine, red);
@@ -175,9 +190,8 @@ __device__ __forceinline__ float coef_of(const ClipFrom& f, double* red) {
     return clip_coef(s, f.max_norm);
 }
 
-template <typename T>
+template <typename LIST>
 __global__ __launch_bounds__(256) void k_list_scale(ListTab t, ClipFrom f) {
-    constexpr int V = VecOf<T>::V;
     __shared__ double red[4];
     const float coef = coef_of(f, red);
     if (coef == 1.f) return;
@@ -185,31 +199,35 @@ __global__ __launch_bounds__(256) void k_list_scale(ListTab t, ClipFrom f) {
     // last is still in the cache in front of the memory (403 M bf16: 273 us forwards, 271 back, and the next norm 5 us less).
     for (long long c = last_chunk(t.chunks); c >= 0; c -= gridDim.x) {
         const int j = find_entry(t, (uint32_t)c);
-        const uint32_t n = t.n[j], at = ((uint32_t)c - t.first[j]) * norm_chunk<T>();
-        T* p = gptr<T>(t.p[j]) + at;
-        const uint32_t left = n - at;
-        if (left >= norm_chunk<T>()) {
-            u32x4 w[kNormVecs];
+        of_type<LIST>(t.n[j], [&](auto type) {
+            using T = decltype(type);
+            constexpr int V = VecOf<T>::V;
+            const uint32_t n = t.n[j] & kCount, at = ((uint32_t)c - t.first[j]) * norm_chunk<T>();
+            T* p = gptr<T>(t.p[j]) + at;
+            const uint32_t left = n - at;
+            if (left >= norm_chunk<T>()) {
+                u32x4 w[kNormVecs];
 #pragma unroll
-            for (int k = 0; k < kNormVecs; ++k) w[k] = *reinterpret_cast<const typename VecOf<T>::vec*>(p + (k * kThreads + threadIdx.x) * V);
+                for (int k = 0; k < kNormVecs; ++k) w[k] = *reinterpret_cast<const typename VecOf<T>::vec*>(p + (k * kThreads + threadIdx.x) * V);
 #pragma unroll
-            for (int k = 0; k < kNormVecs; ++k) {
-                float v[V];
-                unpack16<T>(w[k], v);
+                for (int k = 0; k < kNormVecs; ++k) {
+                    float v[V];
+                    unpack16<T>(w[k], v);
 #pragma unroll
-                for (int i = 0; i < V; ++i) v[i] *= coef;            // in 32 bits, rounded once
-                *reinterpret_cast<typename VecOf<T>::vec*>(p + (k * kThreads + threadIdx.x) * V) = pack16<T>(v);
+                    for (int i = 0; i < V; ++i) v[i] *= coef;        // in 32 bits, rounded once
+                    *reinterpret_cast<typename VecOf<T>::vec*>(p + (k * kThreads + threadIdx.x) * V) = pack16<T>(v);
+                }
+            } else {
+                for (uint32_t o = threadIdx.x * V; o < left; o += kThreads * V) {
+                    float v[V];
+                    const int m = (int)min(left - o, (uint32_t)V);
+                    load_chunk<T>(p + o, m, v);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) v[i] *= coef;
+                    store_chunk<T>(p + o, m, v);
+                }
             }
-        } else {
-            for (uint32_t o = threadIdx.x * V; o < left; o += kThreads * V) {
-                float v[V];
-                const int m = (int)min(left - o, (uint32_t)V);
-                load_chunk<T>(p + o, m, v);
-#pragma unroll
-                for (int i = 0; i < V; ++i) v[i] *= coef;
-                store_chunk<T>(p + o, m, v);
-            }
-        }
+        });
     }
 }
 
@@ -403,37 +421,40 @@ unsigned strided_blocks(const Strided& s) { return (unsigned)std::min<long long>
 
 uint32_t chunk_of(int dtype) { return dtype == FNET_F32 ? norm_chunk<float>() : norm_chunk<bf16_t>(); }
 
-// calls launch(dtype, table) for every table of at most kTab entries of one type; 0 or the first error
+// calls launch(table) for every table of at most kTab entries; 0 or the first error
 template <typename F>
 int for_tables(int n, const uint64_t* ptr, const int64_t* numel, const int32_t* dtype, F launch) {
-    for (int d = 0; d <= FNET_F16; ++d) {
-        ListTab t;
-        t.count = 0;
-        t.chunks = 0;
-        const uint32_t chunk = chunk_of(d);
-        for (int k = 0; k < n; ++k) {
-            if (dtype[k] != d) continue;
-            for (int64_t at = 0; at < numel[k]; at += kMaxEntry) {
-                const uint32_t len = (uint32_t)std::min<int64_t>(numel[k] - at, kMaxEntry);
-                t.p[t.count] = ptr[k] + (uint64_t)at * elem_size(d);
-                t.n[t.count] = len;
-                t.first[t.count] = t.chunks;
-                t.chunks += (len + chunk - 1) / chunk;
-                if (++t.count == kTab) {
-                    const int rc = launch(d, t);
-                    if (rc != FNET_OK) return rc;
-                    t.count = 0;
-                    t.chunks = 0;
-                }
+    ListTab t;
+    t.count = 0;
+    t.chunks = 0;
+    for (int k = 0; k < n; ++k) {
+        const uint32_t chunk = chunk_of(dtype[k]);
+        for (int64_t at = 0; at < numel[k]; at += kMaxEntry) {
+            const uint32_t len = (uint32_t)std::min<int64_t>(numel[k] - at, kMaxEntry);
+            t.p[t.count] = ptr[k] + (uint64_t)at * elem_size(dtype[k]);
+            t.n[t.count] = len | (uint32_t)dtype[k] << 30;
+            t.first[t.count] = t.chunks;
+            t.chunks += (len + chunk - 1) / chunk;
+            if (++t.count == kTab) {
+                const int rc = launch(t);
+                if (rc != FNET_OK) return rc;
+                t.count = 0;
+                t.chunks = 0;
             }
         }
-        if (t.count) {
-            const int rc = launch(d, t);
-            if (rc != FNET_OK) return rc;
-        }
     }
-    return FNET_OK;
+    return t.count ? launch(t) : FNET_OK;
 }
+
+// the type of a list's tensors, -1 for several
+int list_type(int n, const int32_t* dtype) {
+    for (int k = 1; k < n; ++k)
+        if (dtype[k] != dtype[0]) return -1;
+    return n ? dtype[0] : -1;
+}
+#define DISPATCH_LIST(type, ...)                                       \
+    if ((type) < 0) { using LIST = void; __VA_ARGS__; }                \
+    else { DISPATCH_T3(type, { using LIST = T; __VA_ARGS__; }) }
 
 #define DISPATCH_KIND(kind, ...)                                                                  \
     if ((kind) == NORM_2) { constexpr int KIND = NORM_2; __VA_ARGS__; }                            \
@@ -455,14 +476,15 @@ int fnet_list_norm_partials(int32_t n, const uint64_t* host_ptr, const int64_t* 
     // what the launches will use is known before the first of them: nothing is launched if the workspace is too small
     auto blocks_of = [&](const ListTab& t) { return (unsigned)std::max<long long>(1, std::min<long long>(t.chunks, (long long)kMaxBlocks * t.chunks / std::max(total, 1ll))); };
     long long need = 0;
-    for_tables(n, host_ptr, host_numel, host_dtype, [&](int, const ListTab& t) { need += blocks_of(t); return FNET_OK; });
+    for_tables(n, host_ptr, host_numel, host_dtype, [&](const ListTab& t) { need += blocks_of(t); return FNET_OK; });
     for (int k = 0; k < n_strided; ++k) need += strided_blocks(to_strided(host_strided[k]));
     FNET_CHECK_ARG(need <= capacity);
     int used = 0;
-    rc = for_tables(n, host_ptr, host_numel, host_dtype, [&](int d, const ListTab& t) -> int {
+    const int type = list_type(n, host_dtype);
+    rc = for_tables(n, host_ptr, host_numel, host_dtype, [&](const ListTab& t) -> int {
         const unsigned b = blocks_of(t);
         double* clk = used == 0 ? clock : nullptr;
-        DISPATCH_T3(d, DISPATCH_KIND(norm_kind, hipLaunchKernelGGL((k_list_norm<T, KIND>), dim3(b), dim3(kThreads), 0, st, t, partials + used, clk, beta1, beta2)));
+        DISPATCH_LIST(type, DISPATCH_KIND(norm_kind, hipLaunchKernelGGL((k_list_norm<LIST, KIND>), dim3(b), dim3(kThreads), 0, st, t, partials + used, clk, beta1, beta2)));
         FNET_LAUNCH_CHECK();
         used += b;
         return FNET_OK;
@@ -509,8 +531,9 @@ int fnet_list_scale(int32_t n, const uint64_t* host_ptr, const int64_t* host_num
     FNET_CHECK_ARG(norm_kind >= NORM_2 && norm_kind <= NORM_INF && max_norm >= 0.0);
     ClipFrom f{partials, norm, n_partials, norm_kind, max_norm, norm_out};
     hipStream_t st = (hipStream_t)stream;
-    rc = for_tables(n, host_ptr, host_numel, host_dtype, [&](int d, const ListTab& t) -> int {
-        DISPATCH_T3(d, hipLaunchKernelGGL(k_list_scale<T>, dim3(std::min<uint32_t>(t.chunks, kMaxBlocks)), dim3(kThreads), 0, st, t, f));
+    const int type = list_type(n, host_dtype);
+    rc = for_tables(n, host_ptr, host_numel, host_dtype, [&](const ListTab& t) -> int {
+        DISPATCH_LIST(type, hipLaunchKernelGGL(k_list_scale<LIST>, dim3(std::min<uint32_t>(t.chunks, kMaxBlocks)), dim3(kThreads), 0, st, t, f));
         FNET_LAUNCH_CHECK();
         f.norm_out = nullptr;
         return FNET_OK;

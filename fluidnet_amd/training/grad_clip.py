@@ -2,8 +2,8 @@
 
 torch.nn.utils.clip_grad_norm_ as ml/training/trainer.py:192-195 calls it, for the parameters of any module: fp32, bf16 and fp16 gradients
 in one list, dense in any layout or strided views of larger buffers (up to six axes), no elements, odd sizes, any alignment.  (The UNet's own
-parameters lie in one flat buffer; FusedClipAdam clips that inside its step.)  One launch per 240 gradients of a type sums the norm, one per
-240 scales; nothing is copied to the host, so both can be captured into a graph.
+parameters lie in one flat buffer; FusedClipAdam clips that inside its step.)  One launch per 240 gradients, of all types, sums the norm, one
+scales; nothing is copied to the host, so both can be captured into a graph.
 
 Norms are summed in 64 bits in a fixed order: the same gradients give the same bits, and neither a large gradient's square nor the tail of a
 long list is lost.  Clipping multiplies in 32 bits and rounds once.  All gradients must lie on one device (one process per GPU).
