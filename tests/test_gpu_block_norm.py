@@ -5,6 +5,7 @@ import itertools
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import block_norm_ref as ref
 from fluidnet_amd.models.block_norm import MAX_WIDTH, GatedResidual, PreNorm, gated_residual, pre_norm
@@ -155,6 +156,59 @@ def test_no_second_derivative():
     g, = torch.autograd.grad([y, h], [d["x"]], [dy.cuda().requires_grad_(True), dh.cuda()], create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         g.sum().backward()
+
+
+def test_node_is_an_ordinary_one():
+    """What autograd promises of any operation: operands changed in place are noticed, a graph is used up by a backward pass, saved tensors go
+    through hooks (checkpointing among them), subsets of gradients, leaves that appear twice."""
+    t, dy, dh = operands((6, 48), F32, gate="element", scale=True, bias=True)
+    dyg, dhg = dy.cuda(), dh.cuda()
+    names = [n for n in ref.NAMES if n in t]
+
+    def once(d):
+        return call(d, "layer", "tanh", 1.0, 1e-6)
+
+    def grads(d, out, which=names, **kw):
+        return torch.autograd.grad(out, [d[n] for n in which], [dyg, dhg], **kw)
+    d = gpu(t, True)
+    out = once(d)
+    want = grads(d, out, retain_graph=True)
+    for n, g in zip(names, want):
+        assert torch.equal(grads(d, out, [n], retain_graph=True)[0], g), n
+    grads(d, out)
+    with pytest.raises(RuntimeError, match="second time"):
+        grads(d, out)
+    out = once(d)
+    with torch.no_grad():
+        d["branch"].add_(1.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        grads(d, out)
+    d = gpu(t, True)
+    with torch.autograd.graph.save_on_cpu():
+        out = once(d)
+    assert all(torch.equal(a, b) for a, b in zip(grads(d, out), want))
+    out = torch.utils.checkpoint.checkpoint(lambda *v: once({**d, **dict(zip(names, v))}), *(d[n] for n in names), use_reentrant=False)
+    assert all(torch.equal(a, b) for a, b in zip(grads(d, out), want))
+    # x as its own branch: its gradient is the sum of both
+    x, b = d["x"].detach().requires_grad_(), d["x"].detach().clone().requires_grad_()
+    one = torch.autograd.grad(gated_residual(x, x), x, [dyg, dhg])[0]
+    two = torch.autograd.grad(gated_residual(d["x"], b), [d["x"], b], [dyg, dhg])
+    assert torch.equal(one, two[0] + two[1])
+    with torch.inference_mode():
+        y, h = once(gpu(t))
+    assert y.is_inference() and torch.equal(h, out[1].detach())
+
+
+def test_other_transforms_are_refused():
+    x, w = torch.randn(4, 32, device="cuda"), torch.ones(32, device="cuda")
+    with pytest.raises(NotImplementedError, match="forward-mode"), torch.autograd.forward_ad.dual_level():
+        pre_norm(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)), w)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda v: pre_norm(v, w))(x)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda v: pre_norm(v, w).sum())(x)
+    with pytest.raises(TypeError, match="must be a tensor"):
+        pre_norm(x, 1.0)
 
 
 def test_capture_of_a_shape_that_never_ran():
