@@ -74,10 +74,9 @@ def build(force: bool = False, verbose: bool = True) -> str:
     if force or jobs or _stale(LIB, objs):
         # -z defs: an unresolved kernel stub must fail the build here, not the dlopen on the GPU box
         run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-Wl,-z,defs", "-o", LIB, *objs])
-    if force or jobs or _stale(TORCH_OPS, [ops_obj, LIB]):
+    if force or jobs or _stale(TORCH_OPS, [ops_obj]):
         at = _torch_dir()
-        run([CXX, "-shared", "-o", TORCH_OPS, ops_obj, f"-L{at}/lib", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip", "-lamdhip64",
-             f"-L{LIBDIR}", "-lfluidnet_hip", "-Wl,-rpath,$ORIGIN/../lib"])
+        run([CXX, "-shared", "-o", TORCH_OPS, ops_obj, f"-L{at}/lib", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip", "-lamdhip64"])
     return LIB
 
 

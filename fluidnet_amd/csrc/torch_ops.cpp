@@ -28,15 +28,23 @@ using at::Tensor;
 using torch::autograd::Node;
 using torch::autograd::variable_list;
 
-PyObject* g_hip_error = nullptr;              // engine.runtime.FluidNetHipError
+// The entry points used here, of the library that engine.runtime has loaded, and its FluidNetHipError; set by bind()
+struct Library {
+    decltype(&fnet_block_norm_fwd) block_norm_fwd;
+    decltype(&fnet_block_norm_bwd) block_norm_bwd;
+    decltype(&fnet_block_norm_workspace) block_norm_workspace;
+    decltype(&fnet_strerror) strerror;
+    decltype(&fnet_last_hip_error) last_hip_error;
+} g_lib;
+PyObject* g_hip_error = nullptr;
 
 struct HipFailure : std::runtime_error {
     using std::runtime_error::runtime_error;
 };
 void check_rc(int rc, const char* what) {
     if (rc == FNET_OK) return;
-    std::string s = std::string(what) + ": " + fnet_strerror(rc);
-    if (rc == FNET_E_HIP) s += " hipError=" + std::to_string(fnet_last_hip_error());
+    std::string s = std::string(what) + ": " + g_lib.strerror(rc);
+    if (rc == FNET_E_HIP) s += " hipError=" + std::to_string(g_lib.last_hip_error());
     throw HipFailure(s);
 }
 
@@ -227,7 +235,7 @@ Outputs run_forward(const Spec& s, const Tensor (&given)[INPUTS], bool keep) {
     a.y = address(out.y);
     a.h = address(out.h);
     a.stats = address(out.stats);
-    check_rc(fnet_block_norm_fwd(&a, stream_of(in[X])), "fnet_block_norm_fwd");
+    check_rc(g_lib.block_norm_fwd(&a, stream_of(in[X])), "fnet_block_norm_fwd");
     return out;
 }
 
@@ -349,11 +357,11 @@ struct BlockNormBackward : public Node {
         a.dpost_bias = address(out[POST_B]);
         Tensor workspace;                             // partial sums of what is summed over rows
         if (sums) {
-            check_rc(fnet_block_norm_workspace(&a, &a.workspace_bytes), "fnet_block_norm_workspace");
+            check_rc(g_lib.block_norm_workspace(&a, &a.workspace_bytes), "fnet_block_norm_workspace");
             if (a.workspace_bytes) workspace = at::empty({a.workspace_bytes}, in[X].options().dtype(at::kByte));
             a.workspace = address(workspace);
         }
-        check_rc(fnet_block_norm_bwd(&a, stream), "fnet_block_norm_bwd");
+        check_rc(g_lib.block_norm_bwd(&a, stream), "fnet_block_norm_bwd");
         return out;
     }
 };
@@ -386,7 +394,7 @@ Outputs block_norm(const Tensor (&in)[INPUTS], int kind, bool post, bool pre, in
 #define FNET_PY_BEGIN HANDLE_TH_ERRORS try {
 #define FNET_PY_END                                                         \
     } catch (const HipFailure& e) {                                          \
-        PyErr_SetString(g_hip_error ? g_hip_error : PyExc_RuntimeError, e.what()); \
+        PyErr_SetString(g_hip_error, e.what());                              \
         return nullptr;                                                      \
     }                                                                        \
     END_HANDLE_TH_ERRORS
@@ -505,8 +513,14 @@ PyObject* py_adam_fits(PyObject*, PyObject* const* args, Py_ssize_t n) {
     FNET_PY_END
 }
 
-PyObject* py_set_error(PyObject*, PyObject* cls) {
-    Py_XINCREF(cls);
+// bind(error class, addresses of the entry points in Library's order); before anything else
+PyObject* py_bind(PyObject*, PyObject* args) {
+    PyObject* cls;
+    unsigned long long at[5];
+    if (!PyArg_ParseTuple(args, "OKKKKK", &cls, at, at + 1, at + 2, at + 3, at + 4)) return nullptr;
+    g_lib = Library{(decltype(g_lib.block_norm_fwd))at[0], (decltype(g_lib.block_norm_bwd))at[1], (decltype(g_lib.block_norm_workspace))at[2],
+                    (decltype(g_lib.strerror))at[3], (decltype(g_lib.last_hip_error))at[4]};
+    Py_INCREF(cls);
     Py_XDECREF(g_hip_error);
     g_hip_error = cls;
     Py_RETURN_NONE;
@@ -518,7 +532,7 @@ PyMethodDef methods[] = {
     {"addresses", py_addresses, METH_O, nullptr},
     {"marks", py_marks, METH_O, nullptr},
     {"adam_fits", (PyCFunction)(void (*)(void))py_adam_fits, METH_FASTCALL, nullptr},
-    {"set_error", py_set_error, METH_O, nullptr},
+    {"bind", py_bind, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_ops", "Host side of the operators on torch tensors", -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -122,12 +122,13 @@ def torch_ops():
     global _torch_ops
     if _torch_ops is None:
         import torch  # noqa: F401  (its libraries have to be there first)
-        lib()
+        L = lib()
         try:
             from . import _torch_ops as ops
         except ImportError as e:
             raise FluidNetHipError(f"fluidnet_amd/engine/_torch_ops.so does not load ({e}): build it with `python -m fluidnet_amd.build`") from e
-        ops.set_error(FluidNetHipError)
+        ops.bind(FluidNetHipError, *(ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in (
+            "fnet_block_norm_fwd", "fnet_block_norm_bwd", "fnet_block_norm_workspace", "fnet_strerror", "fnet_last_hip_error")))
         _torch_ops = ops
     return _torch_ops
 

@@ -1,7 +1,6 @@
 #!/bin/bash
 # Variant library for A/B runs: tools/build_variant.sh NAME SOURCE.hip "-DFLAG=.. ..."  ->  fluidnet_amd/lib/variants/libfnet_NAME.so
-# (one source recompiled with the extra flags, the other objects taken from the regular build; select with FNET_LIB=...; engine/_torch_ops.so, so the block norms,
-# keeps to the regular library)
+# (one source recompiled with the extra flags, the other objects taken from the regular build; select with FNET_LIB=...)
 set -e
 cd "$(dirname "$0")/.."
 name=$1; src=$2; flags=$3
