@@ -231,14 +231,17 @@ class ClipAdam:
                     if torch.cuda.is_current_stream_capturing():
                         raise RuntimeError("ClipAdam: a parameter was written since the last step; call refresh() before capturing the step")
                     w.copy_(p)
-        have = [k for k, p in enumerate(self.params) if p.grad is not None]
+        lists = (self.params, [p.grad for p in self.params], self._m, self._v, self._w)
+        have = [k for k, g in enumerate(lists[1]) if g is not None]
         if not have:
             return
-        pick = lambda ts: [ts[k] for k in have]  # noqa: E731
-        params = pick(self.params)
-        grads = [p.grad if _same_layout(p, p.grad) else torch.empty_like(p).copy_(p.grad) for p in params]
-        self.grad_norm = clip_adam_(params, grads, pick(self._m), pick(self._v), self._clock, masters=pick(self._w), lr=self._lr, betas=self.betas,
-                                    eps=self.eps, weight_decay=self.weight_decay, max_norm=self.max_norm)
+        if len(have) < len(self.params):
+            lists = [[ts[k] for k in have] for ts in lists]
+        params, grads, m, v, w = lists
+        if not rt.torch_ops().adam_fits(params, grads, m, v, w):
+            grads = [g if _same_layout(p, g) else torch.empty_like(p).copy_(g) for p, g in zip(params, grads)]
+        self.grad_norm = clip_adam_(params, grads, m, v, self._clock, masters=w, lr=self._lr, betas=self.betas, eps=self.eps,
+                                    weight_decay=self.weight_decay, max_norm=self.max_norm)
         self._seen = rt.torch_ops().marks(self.params)
 
     @property
