@@ -478,6 +478,25 @@ def test_large_offsets():
     assert torch.equal(pre_norm(x, w), pre_norm(x.clone(memory_format=torch.contiguous_format), w))
 
 
+def test_more_than_2_31_elements():
+    """Rows behind 2^31 elements, forward and backward, operands of a stride of their own among them: the last rows as if they were alone."""
+    rows, width, last = 265_000, 8192, 3                  # 2.17e9 elements, 4.3 GB each
+    x = torch.empty(rows, width, dtype=BF16, device="cuda").fill_(0.5)
+    tail = torch.randn(last, width, generator=torch.Generator().manual_seed(7)).to(BF16).cuda()
+    x[-last:] = tail
+    w = torch.rand(width, device="cuda")
+    up = torch.full((1, width), 0.25, dtype=BF16, device="cuda").expand(rows, width)
+
+    def run(x, up):
+        x = x.detach().requires_grad_()
+        y, h = gated_residual(x, x.detach(), post_weight=w, pre_weight=w, residual_scale=0.5)
+        return y.detach()[-last:], h.detach()[-last:], torch.autograd.grad([y, h], x, [up, up])[0][-last:]
+    for a, b in zip(run(x, up), run(tail, up[-last:])):
+        assert torch.equal(a, b)
+    del x
+    torch.cuda.empty_cache()
+
+
 def test_modules():
     m = GatedResidual(96, kind="layer", bias=True, scale_init=0.1, channel_gate=0.0, gate_act="tanh").cuda()
     first = PreNorm(96, kind="layer", bias=True).cuda()
