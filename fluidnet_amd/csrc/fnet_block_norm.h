@@ -38,7 +38,7 @@ inline RowLaunch row_launch(int L, int E, int width) {
 // How the rows are cut: segments = samples * parts, part p of a sample its rows [p * part_rows, (p + 1) * part_rows).  With a gate per sample
 // a segment ends with its sample, so that what the gate multiplies is constant over it; otherwise all rows are one "sample".
 struct RowCut {
-    int samples, parts;
+    int samples, parts;          // their product: segments, at most 2^30 and the target
     long long sample_rows, part_rows;
 };
 // about `target` segments, each of at least min_steps steps of rpb rows where there are that many for 256 of them
@@ -49,7 +49,7 @@ inline RowCut cut_rows(const FnetBlockNorm& a, int rpb, long long target, int mi
     c.sample_rows = by_sample ? a.tokens : a.rows;
     const long long steps = (c.sample_rows + rpb - 1) / rpb;
     long long parts = target / c.samples;
-    const long long fill = std::min(steps, (long long)(255 + c.samples) / c.samples);
+    const long long fill = std::min(steps, (255ll + c.samples) / c.samples);
     parts = std::min(parts, std::max(steps / min_steps, fill));
     if (parts < 1) parts = 1;
     c.part_rows = ((steps + parts - 1) / parts) * rpb;

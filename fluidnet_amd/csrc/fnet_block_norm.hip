@@ -10,6 +10,14 @@ namespace {
 bool type_ok(int d, int operand) { return d == FNET_F32 || d == operand; }
 bool aligned(uint64_t p, int dtype) { return p % (dtype == FNET_F32 ? 4 : 2) == 0; }
 
+// The arguments as the kernels take them: a gate per sample of one token is a row of values per row.  (Samples of two tokens and more are at
+// most 2^30, so the kernels' 32-bit count of segments stays below 2^31 when a grid is added to it; samples of one row may be 2^31 - 1.)
+FnetBlockNorm as_launched(const FnetBlockNorm& given) {
+    FnetBlockNorm a = given;
+    if (a.gate_kind == FNET_GATE_SAMPLE && a.tokens == 1) a.gate_kind = FNET_GATE_ELEMENT;
+    return a;
+}
+
 }  // namespace
 
 int fnet_resident_blocks(const void* kernel, int threads, size_t lds, int otherwise) {
@@ -74,7 +82,7 @@ int fnet_block_norm_check(const FnetBlockNorm* a) {
 int fnet_block_norm_fwd(const FnetBlockNorm* host_args, void* stream) {
     const int rc = fnet_block_norm_check(host_args);
     if (rc != FNET_OK) return rc;
-    const FnetBlockNorm& a = *host_args;
+    const FnetBlockNorm a = as_launched(*host_args);
     if (a.rows == 0) return FNET_OK;
     FNET_CHECK_ARG((a.branch != 0) == (a.y != 0) && (a.y != 0 || a.h != 0) && (a.h != 0 || (a.pre_weight == 0 && a.pre_bias == 0)));
     FNET_CHECK_ARG(aligned(a.y | a.h, a.dtype));
@@ -224,7 +232,7 @@ int fnet_block_norm_workspace(const FnetBlockNorm* host_args, int64_t* bytes) {
     *bytes = 0;
     if (host_args->rows == 0) return FNET_OK;
     BwdShape s;
-    DISPATCH_ROW(host_args->width, { bwd_shape(*host_args, L, E, 0, &s); });
+    DISPATCH_ROW(host_args->width, { bwd_shape(as_launched(*host_args), L, E, 0, &s); });
     *bytes = s.bytes;
     return FNET_OK;
 }
@@ -232,7 +240,7 @@ int fnet_block_norm_workspace(const FnetBlockNorm* host_args, int64_t* bytes) {
 int fnet_block_norm_bwd(const FnetBlockNorm* host_args, void* stream) {
     const int rc = bwd_check(host_args);
     if (rc != FNET_OK) return rc;
-    const FnetBlockNorm& a = *host_args;
+    const FnetBlockNorm a = as_launched(*host_args);
     if (a.rows == 0) return FNET_OK;
     FNET_CHECK_ARG((!a.post && !a.dh) || a.stats != 0);
     FNET_CHECK_ARG(a.dh != 0 || (!a.dpre_weight && !a.dpre_bias));
