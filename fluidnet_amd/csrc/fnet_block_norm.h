@@ -21,7 +21,8 @@ struct RowShape {
     // rows of whole waves are the same for all lanes of a wave: their addresses stay in scalar registers
     static __device__ __forceinline__ long long row(long long r) {
         if (!WAVES && L != 64) return r;
-        return (long long)__builtin_amdgcn_readfirstlane((int)r);      // rows < 2^31
+        // r < 2^31 + 4: a block's last groups may lie behind the last row, so the 32 bits that are carried over are unsigned
+        return (long long)(uint32_t)__builtin_amdgcn_readfirstlane((int)r);
     }
 };
 struct RowLaunch {

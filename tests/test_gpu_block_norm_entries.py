@@ -44,3 +44,24 @@ def test_one_token_a_sample_is_a_gate_per_element(rows, width):
     want, got = run(ELEMENT, rows), run(SAMPLE, 1)
     for k in want:
         assert torch.equal(got[k], want[k]), k
+
+
+def test_groups_behind_the_last_of_nearly_2_31_rows():
+    """The last step of the last sample begins at row 2^31 - 3, so its fourth group would have row 2^31, which must be no row at all.  Operands
+    of stride 0 make room for so many rows; only the statistics (34 GB) have a place per row.  Sums of ones: up to 2^24 per lane they are exact,
+    the 4096 partial sums of 2^19 add up with at most 4096 roundings of 2^-24 in order, less than 1e-3 of the sum."""
+    rows, tokens, width = (1 << 31) - 2, 357_913_941, 257          # six samples; tokens % 4 == 1
+    assert rows % tokens == 0 and (rows - tokens) % 4 == 1
+    one = torch.ones(width, device="cuda")
+    stats = torch.ones(4 * rows, device="cuda")
+    out = {"ds": torch.zeros(width, device="cuda"), "dg": torch.zeros(rows // tokens, width, device="cuda")}
+    a = _args(rows, width, one, one, one, out, gk=SAMPLE, tokens=tokens, ga=0, kind=0, a=1.0, dy=one.data_ptr(), stats=stats.data_ptr(), xs=0, bs=0, gs=0, dys=0)
+    n = ctypes.c_int64()
+    L = rt.lib()
+    assert L.fnet_block_norm_workspace(_pack(**a), ctypes.byref(n)) == 0
+    ws = torch.empty(n.value + 16, dtype=torch.uint8, device="cuda")
+    assert L.fnet_block_norm_bwd(_pack(**{**a, "ws": ws.data_ptr(), "wsn": n.value}), rt.raw_stream(0)) == 0
+    torch.cuda.synchronize()
+    assert ((out["ds"].double() - rows).abs() <= 1e-3 * rows).all() and ((out["dg"].double() - tokens).abs() <= 1e-3 * tokens).all()
+    del stats
+    torch.cuda.empty_cache()
