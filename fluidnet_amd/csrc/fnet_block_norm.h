@@ -24,6 +24,11 @@ struct RowShape {
         // r < 2^31 + 4: a block's last groups may lie behind the last row, so the 32 bits that are carried over are unsigned
         return (long long)(uint32_t)__builtin_amdgcn_readfirstlane((int)r);
     }
+    // a value per row, likewise (16 elements a lane: they spill as it is, and 4 to 27 registers go if a wide row's gate becomes a scalar)
+    static __device__ __forceinline__ float row_value(float v) {
+        if ((!WAVES && L != 64) || E > 8) return v;
+        return __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(v)));
+    }
 };
 struct RowLaunch {
     int waves;                   // per row (L = 0)
@@ -201,40 +206,74 @@ __device__ __forceinline__ void store_param(uint64_t p, long long at, bool f32, 
     }
 }
 
-// act(g) and its derivative of a chunk; the choice is uniform, so it stands outside the loops.  Both derivatives are written with
-// e = exp(-|g|) (or its square), which keeps them exact where act(g) is within a rounding of 1.  v_rcp_f32 is good for one unit in the last place.
-__device__ __forceinline__ float gate_value(float g, int act) {
-    if (act == FNET_GATE_SIGMOID) return __builtin_amdgcn_rcpf(1.f + __expf(-g));
+// act(g) and its derivative; the choices are uniform, so they stand outside the loops.  Both derivatives are written with e = exp(-|g|) (or its
+// square), which keeps them exact where act(g) is within a rounding of 1.
+// exp(v), v <= 0, in 32 bits: 2^n with n the rounded v / ln 2, and 1 + t for the rest t = v - n ln 2, with ln 2 in two parts (Cody and Waite's
+// reduction, without the rounding to a whole n).  v_exp_f32 is good for one unit in the last place.  Below -200 the result is 0 all the same,
+// and an infinity must not meet itself in t; a NaN passes the comparison.
+__device__ __forceinline__ float gate_exp(float v) {
+    v = v < -200.f ? -200.f : v;
+    const float n = v * 1.44269504f, p = __builtin_amdgcn_exp2f(n), t = fmaf(n, 1.90465421e-9f, fmaf(n, -0.693147182f, v));
+    return fmaf(p, t, p);
+}
+// 1 / d for d in 1 .. 4, one Newton step behind v_rcp_f32
+__device__ __forceinline__ float gate_rcp(float d) {
+    const float r = __builtin_amdgcn_rcpf(d);
+    return fmaf(fmaf(-d, r, 1.f), r, r);
+}
+// fp32 gates take these, and so do all gates per row (one value a row costs nothing).  Other 16-bit gates take the GPU's own power of two and
+// reciprocal alone, whose rounded exponent is off by |g| 2^-24 (1e-6 of a sigmoid at -16): their gradient and the 16-bit outputs round that away,
+// and a gate per element would pay for more (16 M bf16 elements with an fp32 gate each: backward 4 to 7 % slower this way).
+__device__ __forceinline__ float gate_value(float g, int act, bool f32) {
+    if (act == FNET_GATE_SIGMOID) {
+        if (!f32) return __builtin_amdgcn_rcpf(1.f + __expf(-g));
+        const float e = gate_exp(-fabsf(g)), r = gate_rcp(1.f + e);
+        return g < 0.f ? e * r : r;
+    }
     if (act == FNET_GATE_TANH) return tanhf(g);
     return g;
 }
-__device__ __forceinline__ float gate_slope(float g, int act) {
+__device__ __forceinline__ float gate_slope(float g, int act, bool f32) {
     if (act == FNET_GATE_IDENTITY) return 1.f;
-    const float e = __expf(act == FNET_GATE_SIGMOID ? -fabsf(g) : -2.f * fabsf(g)), r = __builtin_amdgcn_rcpf(1.f + e);
-    return (act == FNET_GATE_SIGMOID ? e : 4.f * e) * r * r;
+    const float v = act == FNET_GATE_SIGMOID ? -fabsf(g) : -2.f * fabsf(g), e = f32 ? gate_exp(v) : __expf(v), n = act == FNET_GATE_SIGMOID ? e : 4.f * e, d = 1.f + e;
+    if (f32) return n * gate_rcp(d * d);
+    const float r = __builtin_amdgcn_rcpf(d);
+    return n * r * r;
 }
-template <int V>
-__device__ __forceinline__ void gate_values(float* g, int act) {
+// of a chunk
+template <int V, bool F32>
+__device__ __forceinline__ void gate_values_of(float* g, int act) {
     if (act == FNET_GATE_SIGMOID) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) g[i] = gate_value(g[i], FNET_GATE_SIGMOID);
+        for (int i = 0; i < V; ++i) g[i] = gate_value(g[i], FNET_GATE_SIGMOID, F32);
     } else if (act == FNET_GATE_TANH) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) g[i] = gate_value(g[i], FNET_GATE_TANH);
+        for (int i = 0; i < V; ++i) g[i] = gate_value(g[i], FNET_GATE_TANH, F32);
     }
 }
-template <int V>
-__device__ __forceinline__ void gate_slopes(float* g, int act) {
+template <int V, bool F32>
+__device__ __forceinline__ void gate_slopes_of(float* g, int act) {
     if (act == FNET_GATE_SIGMOID) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) g[i] = gate_slope(g[i], FNET_GATE_SIGMOID);
+        for (int i = 0; i < V; ++i) g[i] = gate_slope(g[i], FNET_GATE_SIGMOID, F32);
     } else if (act == FNET_GATE_TANH) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) g[i] = gate_slope(g[i], FNET_GATE_TANH);
+        for (int i = 0; i < V; ++i) g[i] = gate_slope(g[i], FNET_GATE_TANH, F32);
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) g[i] = 1.f;
     }
+}
+// V = 4: the operands are fp32 and so is the gate
+template <int V>
+__device__ __forceinline__ void gate_values(float* g, int act, bool f32) {
+    if (V == 4 || f32) gate_values_of<V, true>(g, act);
+    else gate_values_of<V, false>(g, act);
+}
+template <int V>
+__device__ __forceinline__ void gate_slopes(float* g, int act, bool f32) {
+    if (V == 4 || f32) gate_slopes_of<V, true>(g, act);
+    else gate_slopes_of<V, false>(g, act);
 }
 
 // How the gate enters a kernel: constant over a segment's rows (none, per channel, per sample: part of the weights), one value per row, or a

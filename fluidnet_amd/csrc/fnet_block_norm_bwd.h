@@ -1,5 +1,7 @@
 // The backward kernel of the norms around a residual block, for one operand type; fnet_block_norm_{f32,bf16,f16}.hip instantiate it.
 #pragma once
+#include <type_traits>
+
 #include "fnet_block_norm.h"
 
 // gradients that are sums over rows
@@ -13,9 +15,16 @@ struct BwdPlan {
     int in_turn;                 // a sample's rows are dealt to its parts in turn; otherwise each part is a run of rows
 };
 
-// Waves per SIMD that the kernel is compiled for: 4 leave 128 registers to each; two more sums or a gate in registers do not fit those, and
-// 3 waves without spilling are faster than 4 with it.  Blocks of more than 8 waves leave no choice.
-constexpr int bwd_waves(int L, int gm, bool bias) { return (bias || gm == GM_VECTOR) && L != 0 ? 3 : 4; }
+// Waves per SIMD that the kernel is compiled for.  4 leave 128 registers to each; two more sums or a gate in registers do not fit those, and
+// 3 waves without spilling are faster than 4 with it.  Two exceptions are told so where the compiler would take one or two registers more:
+// 16-bit rows of 8 lanes, and bf16 rows of 16 without biases (16 M elements, 100 wide, a gate per element: 87 us with 3 waves, 79 with 4).
+// L = 0 is one kernel for blocks of 5 to 16 waves and has to be compiled for 16, which is 128 registers: of up to 8192 elements a row the forms
+// with biases spill 8 to 33 registers and those with a gate per element alone up to 8, wider rows 57 to 167 without biases and 219 to 395 with.
+template <typename T>
+constexpr int bwd_waves(int L, int gm, bool bias) {
+    if (L == 0 || (L == 8 && gm != GM_VECTOR && sizeof(T) == 2) || (L == 16 && !bias && std::is_same<T, bf16_t>::value)) return 4;
+    return bias || gm == GM_VECTOR ? 3 : 4;
+}
 
 // arrays of weights that the kernel keeps in the LDS; rows of more than 8192 elements leave no room for the third
 constexpr int bwd_lds_arrays(int E, bool bias) { return bias && E == 8 ? 3 : 2; }
@@ -38,7 +47,7 @@ namespace {
 // when they are left: f is part of W and B, and dgate of a channel or sample comes from the same two sums.
 // A row's arithmetic is 18 to 40 operations an element, which keeps it below the time of the 10 to 14 bytes it moves (bf16).
 template <typename T, int L, int E, int GM, bool LAYER, bool BIAS>
-__global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, BIAS)) void k_block_norm_bwd(FnetBlockNorm a, BwdPlan plan, RowLaunch rl) {
+__global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves<T>(L, GM, BIAS)) void k_block_norm_bwd(FnetBlockNorm a, BwdPlan plan, RowLaunch rl) {
     using S = RowShape<T, L, E>;
     constexpr int V = S::V, K = S::K;
     constexpr bool WY_LDS = bwd_lds_arrays(E, BIAS) == (BIAS ? 3 : 2);
@@ -101,7 +110,7 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
             for (int i = 0; i < V; ++i) s[i] *= a.residual_scale;
             if (GM == GM_CONST && a.gate) {
                 load_param_or<T, S::TINY>(a.gate, gate_at + col[k], gf, left[k], 1.f, w);
-                gate_values<V>(w, a.gate_act);
+                gate_values<V>(w, a.gate_act, gf);
 #pragma unroll
                 for (int i = 0; i < V; ++i) s[i] *= w[i];
             }
@@ -176,13 +185,13 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
             const float p1 = weights[W_O * pitch + c], p0 = BIAS ? weights[W_B * pitch + c] : 0.f;
             const float sc = a.residual_scale * (a.scale ? load_param1<T>(a.scale, c, pf) : 1.f);
             const float g = GM == GM_CONST && a.gate ? load_param1<T>(a.gate, gate_at + c, gf) : 0.f;
-            const float f = GM == GM_CONST && a.gate ? gate_value(g, a.gate_act) : 1.f;
+            const float f = GM == GM_CONST && a.gate ? gate_value(g, a.gate_act, gf) : 1.f;
             if (plan.dst[SUM_POST_W]) leave_more(SUM_POST_W, more, c, sc * f * p1);
             if (BIAS && plan.dst[SUM_POST_B]) leave_more(SUM_POST_B, more, c, sc * f * p0);
             if (plan.dst[SUM_SCALE] || plan.dst[SUM_GATE]) {
                 const float u = (a.post_weight ? load_param1<T>(a.post_weight, c, pf) : 1.f) * p1 + (BIAS && a.post_bias ? load_param1<T>(a.post_bias, c, pf) * p0 : 0.f);
                 if (plan.dst[SUM_SCALE]) leave_more(SUM_SCALE, more, c, a.residual_scale * f * u);
-                if (plan.dst[SUM_GATE]) leave(SUM_GATE, seg, c, sc * gate_slope(g, a.gate_act) * u, gf);
+                if (plan.dst[SUM_GATE]) leave(SUM_GATE, seg, c, sc * gate_slope(g, a.gate_act, gf) * u, gf);
             }
         }
     };
@@ -238,7 +247,7 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
             Row now;
             load(row, here, now);
             const float mu_o = now.mu_o, r_o = now.r_o, mu_y = now.mu_y, r_y = now.r_y, gt = now.gate;
-            const float ft = GM == GM_ROW ? gate_value(gt, a.gate_act) : 1.f;
+            const float ft = GM == GM_ROW ? S::row_value(gate_value(gt, a.gate_act, true)) : 1.f;
             float z[K][V], d[K][V], f[GM == GM_VECTOR ? K : 1][V];
 #pragma unroll
             for (int k = 0; k < K; ++k) {
@@ -246,7 +255,7 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
                 if (GM == GM_VECTOR) {
                     float(&fk)[V] = f[GM == GM_VECTOR ? k : 0];
                     load_param_or<T, S::TINY>(a.gate, row * a.gate_stride + col[k], gf, here ? left[k] : 0, 0.f, fk);
-                    gate_values<V>(fk, a.gate_act);
+                    gate_values<V>(fk, a.gate_act, gf);
                 }
                 if (post) {
 #pragma unroll
@@ -321,7 +330,7 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
                         if (a.dgate) {
                             float g[V];
                             load_param_or<T, S::TINY>(a.gate, row * a.gate_stride + col[k], gf, here ? left[k] : 0, 0.f, g);
-                            gate_slopes<V>(g, a.gate_act);
+                            gate_slopes<V>(g, a.gate_act, gf);
 #pragma unroll
                             for (int i = 0; i < V; ++i) {
                                 if (i % 4 == 0) {
@@ -353,7 +362,7 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS), bwd_waves(L, GM, 
                 }
                 if (post || GM == GM_ROW) sum(s3, at);
                 if (GM == GM_ROW && a.dgate && here && at.lane == 0) {
-                    const float dg = gate_slope(gt, a.gate_act) * (s3[1] + s3[2]);
+                    const float dg = gate_slope(gt, a.gate_act, true) * (s3[1] + s3[2]);
                     if (gf) gptr<float>(a.dgate)[row] = dg;
                     else gptr<T>(a.dgate)[row] = f_to_elem<T>(dg);
                 }

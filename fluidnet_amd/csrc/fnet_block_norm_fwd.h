@@ -45,7 +45,7 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS)) void k_block_norm
             if ((GM == GM_CONST || GM == GM_SAMPLE) && a.gate) {
                 float g[V];
                 load_param_or<T, S::TINY>(a.gate, gate_at + col[k], gf, left[k], 1.f, g);
-                gate_values<V>(g, a.gate_act);
+                gate_values<V>(g, a.gate_act, gf);
 #pragma unroll
                 for (int i = 0; i < V; ++i) s[i] *= g[i];
             }
@@ -141,7 +141,7 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS)) void k_block_norm
         }
         if (have_branch) {
             float r = 1.f, mu = 0.f;
-            if (GM == GM_ROW) gt = gate_value(gt, a.gate_act);
+            if (GM == GM_ROW) gt = S::row_value(gate_value(gt, a.gate_act, true));
             if (post) {
                 r = normalise(o, mu);
                 if (a.stats && here && at.lane == 0) {
@@ -151,7 +151,7 @@ __global__ __launch_bounds__((RowShape<T, L, E>::MAX_THREADS)) void k_block_norm
             }
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                if (GM == GM_VECTOR) gate_values<V>(g[GM == GM_VECTOR ? k : 0], a.gate_act);
+                if (GM == GM_VECTOR) gate_values<V>(g[GM == GM_VECTOR ? k : 0], a.gate_act, gf);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     o[k][i] = BIAS ? fmaf(o[k][i] * r, wo[k][i], bo[BIAS ? k : 0][i]) : o[k][i] * r * wo[k][i];
