@@ -28,6 +28,8 @@ _STRIDED = struct.Struct("=Q2i12q")
 
 def _collapsed(t: torch.Tensor):
     """Sizes and strides of a tensor's memory, largest stride first, neighbouring axes merged; None if elements share memory."""
+    if t.numel() == 0:
+        return [[1, 0]]
     axes = sorted(((st, n) for n, st in zip(t.shape, t.stride()) if n != 1), reverse=True)
     out: List[List[int]] = []
     for st, n in axes:
