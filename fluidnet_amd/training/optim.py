@@ -184,7 +184,7 @@ class ClipAdam:
                 raise ValueError(f"parameter {k} must be dense (shape {tuple(p.shape)}, strides {p.stride()})")
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("ClipAdam: make one eager step before capturing one")
-        old = self.state_dict() if self._m is not None else None          # the module was moved to another device
+        old = self._packed() if self._m is not None else None          # the module was moved to another device
         self._m = [torch.zeros_like(p, dtype=torch.float32) for p in self.params]
         self._v = [torch.zeros_like(p, dtype=torch.float32) for p in self.params]
         self._w = [None if p.dtype is torch.float32 else p.detach().float() for p in self.params]
@@ -250,6 +250,9 @@ class ClipAdam:
 
     def state_dict(self) -> Dict:
         self._init_state()
+        return self._packed()
+
+    def _packed(self) -> Dict:
         cpu = lambda ts: [None if t is None else t.detach().cpu() for t in ts]  # noqa: E731
         return {"step": self.step_count, "lr": self.param_groups[0]["lr"], "exp_avg": cpu(self._m), "exp_avg_sq": cpu(self._v),
                 "master": cpu(self._w), "betas": self.betas, "eps": self.eps, "max_norm": self.max_norm, "weight_decay": self.weight_decay}

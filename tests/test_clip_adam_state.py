@@ -34,3 +34,26 @@ def test_parameters_that_are_not_dense_are_refused(host):
         assert p.stride() == view.stride()
         with pytest.raises(ValueError, match="must be dense"):
             ClipAdam([p], 1e-3)._init_state()
+
+
+def test_state_follows_a_module_to_another_device(host, monkeypatch):
+    params = _params((3, 2), (4,), dtype=torch.bfloat16)
+    opt = ClipAdam(params, 1e-3, betas=(0.8, 0.9))
+    opt._init_state()
+    for k in range(2):
+        opt._m[k].fill_(0.25 + k)
+        opt._v[k].fill_(0.5 + k)
+        opt._w[k].mul_(1 + 1e-4)           # still rounds to its parameter
+    opt._clock.copy_(torch.tensor([3.0, 0.8 ** 3, 0.9 ** 3], dtype=torch.float64))
+    opt.param_groups[0]["lr"] = 7e-4
+    opt.push_lr()
+    kept = {n: [t.clone() for t in getattr(opt, n)] for n in ("_m", "_v", "_w")}
+    # the clock claims to lie on another device than the parameters, as it does after a move; the move itself would need two GPUs
+    class Elsewhere(torch.Tensor):
+        device = torch.device("meta")
+    opt._clock = opt._clock.as_subclass(Elsewhere)
+    opt._init_state()
+    assert type(opt._clock) is torch.Tensor and opt._clock.device == params[0].device
+    for n, ts in kept.items():
+        assert all(torch.equal(a, b) for a, b in zip(getattr(opt, n), ts)), n
+    assert opt.step_count == 3 and opt._clock.tolist() == [3.0, 0.8 ** 3, 0.9 ** 3] and float(opt._lr) == 7e-4
