@@ -260,8 +260,12 @@ class ClipAdam:
     @torch.no_grad()
     def load_state_dict(self, sd: Dict) -> None:
         self._init_state()
-        if len(sd["exp_avg"]) != len(self.params):
-            raise ValueError(f"the state is of {len(sd['exp_avg'])} parameters, this optimizer has {len(self.params)}")
+        for name in ("exp_avg", "exp_avg_sq", "master"):
+            if len(sd[name]) != len(self.params):
+                raise ValueError(f"the state's {name} is of {len(sd[name])} parameters, this optimizer has {len(self.params)}")
+            for k, (t, p) in enumerate(zip(sd[name], self.params)):
+                if (t is not None or name != "master") and t.shape != p.shape:
+                    raise ValueError(f"the state's {name} {k} has shape {tuple(t.shape)}, the parameter {tuple(p.shape)}")
         t = int(sd["step"])
         self._clock.copy_(torch.tensor([t, self.betas[0] ** t, self.betas[1] ** t], dtype=torch.float64))
         self.param_groups[0]["lr"] = float(sd["lr"])

@@ -57,3 +57,42 @@ def test_state_follows_a_module_to_another_device(host, monkeypatch):
     for n, ts in kept.items():
         assert all(torch.equal(a, b) for a, b in zip(getattr(opt, n), ts)), n
     assert opt.step_count == 3 and opt._clock.tolist() == [3.0, 0.8 ** 3, 0.9 ** 3] and float(opt._lr) == 7e-4
+
+
+def _state(opt):
+    return [t.clone() for ts in (opt._m, opt._v, opt._w) for t in ts if t is not None] + [opt._clock.clone(), opt._lr.clone()]
+
+
+@pytest.mark.parametrize("wrong", [
+    lambda sd: sd["exp_avg"].__setitem__(0, torch.ones(1, 2)),                    # would be broadcast over the rows
+    lambda sd: sd["exp_avg_sq"].__setitem__(1, torch.ones(())),                   # would be broadcast over everything
+    lambda sd: sd["exp_avg"].__setitem__(1, torch.ones(5)),
+    lambda sd: sd["master"].__setitem__(0, torch.ones(2)),
+    lambda sd: sd["exp_avg_sq"].pop(),
+    lambda sd: sd["master"].pop(),
+    lambda sd: sd["exp_avg"].append(torch.ones(4)),
+])
+def test_states_of_other_parameters_are_refused(host, wrong):
+    """Before anything of the optimizer's own is written."""
+    opt = ClipAdam(_params((3, 2), (4,), dtype=torch.bfloat16), 1e-3)
+    opt._init_state()
+    before, sd = _state(opt), opt.state_dict()
+    sd["step"], sd["lr"] = 9, 5e-2
+    wrong(sd)
+    with pytest.raises(ValueError, match="parameter"):
+        opt.load_state_dict(sd)
+    assert opt.step_count == 0 and opt.param_groups[0]["lr"] == 1e-3
+    assert all(torch.equal(a, b) for a, b in zip(before, _state(opt)))
+
+
+def test_a_state_loads_into_other_types_and_layouts(host):
+    """fp32 parameters take the moments of bf16 ones and ignore their masters; the other way round the master is the parameter."""
+    a, b = ClipAdam(_params((3, 2), dtype=torch.bfloat16), 1e-3), ClipAdam(_params((3, 2)), 1e-3)
+    for opt in (a, b):
+        opt._init_state()
+    a._m[0].fill_(0.5)
+    b.load_state_dict(a.state_dict())
+    assert torch.equal(b._m[0], a._m[0]) and b._w == [None]
+    b._m[0].fill_(0.25)
+    a.load_state_dict(b.state_dict())
+    assert torch.equal(a._m[0], b._m[0]) and torch.equal(a._w[0], a.params[0].detach().float())

@@ -25,3 +25,25 @@ def test_parameters_of_no_elements(dtype):
     opt = ClipAdam(only, 1e-2, max_norm=0.3)
     opt.step()
     assert float(opt.grad_norm) == 0.0 and opt.step_count == 1
+
+
+def test_a_loaded_state_goes_on():
+    """Saved after three steps and loaded into a new optimizer of the same parameters, the next step is the same, bit for bit."""
+    g = torch.Generator().manual_seed(3)
+    start = [torch.randn(s, generator=g) for s in ((9, 4), (130,), (2, 0))]
+    grads = [[torch.randn(p.shape, generator=g) for p in start] for _ in range(4)]
+    ends = []
+    for again in (False, True):
+        ps = [torch.nn.Parameter(p.cuda().bfloat16()) for p in start]
+        opt = ClipAdam(ps, 1e-2, max_norm=1.0)
+        for k, gs in enumerate(grads):
+            for p, v in zip(ps, gs):
+                p.grad = v.cuda().bfloat16()
+            if again and k == 3:
+                sd, opt = opt.state_dict(), ClipAdam(ps, 1e-2, max_norm=1.0)
+                opt.load_state_dict(sd)
+            opt.step()
+        ends.append([*(p.detach() for p in ps), *opt._m, *opt._v, *opt._w])
+    assert all(torch.equal(a, b) for a, b in zip(*ends))
+    with pytest.raises(ValueError, match="shape"):
+        ClipAdam([torch.nn.Parameter(torch.zeros(9, 1, device="cuda")), *ps[1:]], 1e-2).load_state_dict(sd)
