@@ -513,6 +513,25 @@ PyObject* py_adam_fits(PyObject*, PyObject* const* args, Py_ssize_t n) {
     FNET_PY_END
 }
 
+// written(params, exp_avgs, exp_avg_sqs, masters, clock): tells autograd of an Adam step in place.  Masters of fp32 parameters are not written.
+PyObject* py_written(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    FNET_PY_BEGIN
+    TORCH_CHECK_TYPE(n == 5 && THPVariable_Check(args[4]), "written takes 4 lists and a tensor");
+    const auto bump = [](const Tensor& t) {
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    };
+    const List params(args[0]), m(args[1]), v(args[2]), masters(args[3]);
+    for (Py_ssize_t k = 0; k < params.size(); ++k) {
+        bump(params[k]);
+        bump(m[k]);
+        bump(v[k]);
+        if (params[k].scalar_type() != at::kFloat) bump(masters[k]);
+    }
+    bump(THPVariable_Unpack(args[4]));
+    Py_RETURN_NONE;
+    FNET_PY_END
+}
+
 // bind(error class, addresses of the entry points in Library's order); before anything else
 PyObject* py_bind(PyObject*, PyObject* args) {
     PyObject* cls;
@@ -532,6 +551,7 @@ PyMethodDef methods[] = {
     {"addresses", py_addresses, METH_O, nullptr},
     {"marks", py_marks, METH_O, nullptr},
     {"adam_fits", (PyCFunction)(void (*)(void))py_adam_fits, METH_FASTCALL, nullptr},
+    {"written", (PyCFunction)(void (*)(void))py_written, METH_FASTCALL, nullptr},
     {"bind", py_bind, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -146,7 +146,7 @@ def clip_adam_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
                    0 if ws is None else ws.data_ptr(), clock.data_ptr(), lr.data_ptr() if isinstance(lr, torch.Tensor) else 0,
                    0 if total is None else total.data_ptr(), 0 if ws is None else lst.capacity)
     rt.call_on(lst.first, "fnet_list_adam", n, address[0], lst.ptrs, address[1], address[2], address[3], lst.numels, lst.codes, a)
-    torch.autograd.graph.increment_version(params)
+    ops.written(params, exp_avgs, exp_avg_sqs, masters, clock)
     return total
 
 
