@@ -545,6 +545,13 @@ int fnet_list_scale(int32_t n, const uint64_t* host_ptr, const int64_t* host_num
         FNET_LAUNCH_CHECK();
         f.norm_out = nullptr;
     }
+    if (f.norm_out) {                                // nothing to scale: one block stores the norm
+        ListTab t;
+        t.count = 0;
+        t.chunks = 0;
+        hipLaunchKernelGGL(k_list_scale<float>, dim3(1), dim3(kThreads), 0, st, t, f);
+        FNET_LAUNCH_CHECK();
+    }
     return FNET_OK;
 }
 

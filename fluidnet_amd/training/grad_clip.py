@@ -160,8 +160,6 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     else:
         ws, used = lst.partials(kind)
         total = torch.empty((), dtype=torch.float32, device=lst.first.device)
-        if used == 0:
-            total.zero_()                       # only gradients of no elements
         _scale(lst, max_norm, kind, ws.data_ptr(), used, 0, total.data_ptr())
     torch.autograd.graph.increment_version(grads)
     return total

@@ -323,7 +323,8 @@ int fnet_block_norm_workspace(const FnetBlockNorm* host_args, int64_t* bytes);
  *   fnet_list_clock          advances clock = (t, beta1^t, beta2^t) alone
  *   fnet_list_norm_finish    the norm itself from the partials
  *   fnet_list_scale          g *= min(1, max_norm / (norm + 1e-6)), the norm taken from the partials, or from *norm if those are 0; the
- *                            norm is also stored to *norm_out if that is not 0.  FNET_E_OVERLAP if two dense tensors share memory
+ *                            norm is also stored to *norm_out if that is not 0, for a list of no elements too.  FNET_E_OVERLAP if two
+ *                            dense tensors share memory
  *   fnet_list_adam           one whole step: norm, clock, update.  Parameters that are not fp32 have an fp32 master that is updated and of
  *                            which they are the rounding.  FNET_E_OVERLAP if what is written shares memory, with itself or with a gradient
  */
