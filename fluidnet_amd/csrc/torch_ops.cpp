@@ -300,7 +300,9 @@ struct BlockNormBackward : public Node {
     torch::autograd::SavedVariable saved[INPUTS], stats;
 
     std::string name() const override { return "BlockNormBackward"; }
+    // mutex_ guards what is saved, as in torch's own nodes: a backward pass on one thread may release it while another one reads it
     void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
         for (auto& v : saved) v.reset_data();
         stats.reset_data();
     }
@@ -318,9 +320,12 @@ struct BlockNormBackward : public Node {
         variable_list out(INPUTS);
         Tensor dy = has_y ? grads[0] : Tensor(), dh = spec.pre ? grads[has_y ? 1 : 0] : Tensor();
         if (!dy.defined() && !dh.defined()) return out;
-        Tensor in[INPUTS];
-        for (int i = 0; i < INPUTS; ++i) in[i] = saved[i].unpack();
-        const Tensor st = stats.unpack();
+        Tensor in[INPUTS], st;
+        {
+            std::lock_guard<std::mutex> lock(mutex_);
+            for (int i = 0; i < INPUTS; ++i) in[i] = saved[i].unpack();
+            st = stats.unpack();
+        }
         at::AutoDispatchBelowADInplaceOrView below;
         FnetBlockNorm a = spec.a;
         c10::DeviceGuard guard(in[X].device());
