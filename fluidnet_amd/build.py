@@ -54,10 +54,10 @@ def build(force: bool = False, verbose: bool = True) -> str:
         src = os.path.join(CSRC, s)
         obj = os.path.join(LIBDIR, s.replace(".hip", ".o"))
         objs.append(obj)
-        if force or _stale(obj, [src] + HEADERS):
+        if force or _stale(obj, [src, __file__] + HEADERS):      # the flags stand in this file
             jobs.append([hipcc, *FLAGS, "-c", src, "-o", obj])
     ops_obj = os.path.join(LIBDIR, "torch_ops.o")
-    if force or _stale(ops_obj, [TORCH_OPS_SRC, HEADERS[-1]]):
+    if force or _stale(ops_obj, [TORCH_OPS_SRC, __file__, HEADERS[-1]]):
         jobs.append([CXX, *_torch_flags(), "-c", TORCH_OPS_SRC, "-o", ops_obj])
 
     def run(cmd):
