@@ -60,3 +60,15 @@ def test_other_flags_are_a_change(compiled):
     compiled()
     assert sorted(compiled(touch="build.py")) == compiled.everything
     assert compiled() == []
+
+
+def test_the_entry_point_compiles_every_time(monkeypatch):
+    import __graft_entry__ as entry
+    asked = []
+
+    def fake(force=False, verbose=True):
+        asked.append(force)
+        return b.LIB
+    monkeypatch.setattr(b, "build", fake)
+    entry.build()
+    assert asked == [True]
