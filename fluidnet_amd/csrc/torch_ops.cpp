@@ -15,7 +15,6 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 
-#include <mutex>
 #include <string>
 #include <unordered_set>
 #include <vector>
@@ -239,19 +238,6 @@ Outputs run_forward(const Spec& s, const Tensor (&given)[INPUTS], bool keep) {
     return out;
 }
 
-// Nodes of graphs that are alive and were made on the default stream
-std::mutex g_default_mutex;
-std::vector<std::weak_ptr<Node>> g_default_nodes;
-size_t g_default_prune = 64;
-
-void note_default_stream(const std::shared_ptr<Node>& node) {
-    std::lock_guard<std::mutex> lock(g_default_mutex);
-    if (g_default_nodes.size() >= g_default_prune) {
-        g_default_nodes.erase(std::remove_if(g_default_nodes.begin(), g_default_nodes.end(), [](const auto& w) { return w.expired(); }), g_default_nodes.end());
-        g_default_prune = std::max<size_t>(64, 2 * g_default_nodes.size());
-    }
-    g_default_nodes.push_back(node);
-}
 // the nodes of leaves in the graph below `node`
 std::unordered_set<Node*> leaves_below(Node* node) {
     std::unordered_set<Node*> seen{node}, leaves;
@@ -268,29 +254,18 @@ std::unordered_set<Node*> leaves_below(Node* node) {
     }
     return leaves;
 }
-// While a graph is captured: refuses if a leaf's gradient would be ordered after the default stream, where its node was made
+// While a graph is captured: refuses if a leaf's gradient would be ordered after the default stream, where its node was made.  A leaf's node
+// lives as long as any graph (of whatever operation) or anyone else holds it.
 void check_capture(Node* node) {
-    std::vector<std::weak_ptr<Node>> eager;
-    {
-        std::lock_guard<std::mutex> lock(g_default_mutex);
-        eager = g_default_nodes;
-    }
     const auto* info = torch::autograd::get_current_graph_task_exec_info();
-    std::unordered_set<Node*> wanted;
     for (Node* leaf : leaves_below(node)) {
         if (info && !info->empty()) {
             const auto it = info->find(leaf);
             if (it == info->end() || !it->second.should_execute()) continue;
         }
-        wanted.insert(leaf);
-    }
-    if (wanted.empty()) return;
-    for (const auto& w : eager) {
-        const std::shared_ptr<Node> other = w.lock();
-        if (!other) continue;
-        for (Node* leaf : leaves_below(other.get()))
-            TORCH_CHECK(!wanted.count(leaf), "outputs of an earlier call from the same leaves, made on the default stream, are alive: drop them before "
-                                             "capturing a backward pass");
+        const auto made_on = leaf->stream();
+        TORCH_CHECK(!made_on || made_on->id() != 0, "outputs of an earlier call from the same leaves, made on the default stream, are alive: drop them "
+                                                    "before capturing a backward pass");
     }
 }
 
@@ -392,7 +367,6 @@ Outputs block_norm(const Tensor (&in)[INPUTS], int kind, bool post, bool pre, in
     if (out.stats.defined()) node->stats = torch::autograd::SavedVariable(out.stats, false);
     if (out.y.defined()) torch::autograd::set_history(out.y, node);
     if (out.h.defined()) torch::autograd::set_history(out.h, node);
-    if (!stream_of(in[X])) note_default_stream(node);
     return out;
 }
 

@@ -21,10 +21,11 @@ all in x's type.  gate, in fp32 or x's type: like x (a value per element), [...,
 or [C] (per channel); gate_act "identity", "sigmoid" or "tanh".  A NaN or infinity stays in its row (and in the sums over rows).
 There is no CPU fallback, and no second derivative (asking for one raises).
 
-Both directions can be captured into a graph.  A captured backward pass that hands gradients to leaves (into .grad or out of
-torch.autograd.grad) raises while outputs of an eager call from the same leaves on the default stream are alive: torch orders a leaf's gradient
-after the stream on which the leaf was first used, the default stream cannot take part in a capture, and the process would end.  Drop those
-outputs first, or make the eager calls on a side stream.  (Outputs of other operations on the same leaves are the caller's to drop.)
+Both directions can be captured into a graph, the backward pass together with its forward pass.  A captured backward pass that hands gradients
+to leaves (into .grad or out of torch.autograd.grad) raises while anything holds a leaf's node that was made on the default stream: outputs of
+an eager call on the same leaves, of these operators or of any other, or a gradient edge.  torch orders a leaf's gradient after the stream on
+which its node was made, the default stream cannot take part in a capture, and the process would end.  Drop those outputs first, or make the
+eager calls on a side stream.
 """
 from __future__ import annotations
 
