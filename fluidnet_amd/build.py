@@ -22,7 +22,8 @@ SOURCES = ["fnet_elementwise.hip", "fnet_loss.hip", "fnet_conv_ref.hip", "fnet_c
 HEADERS = [os.path.join(CSRC, h) for h in ("fnet_common.h", "fnet_vec.h", "fnet_block_norm.h", "fnet_block_norm_fwd.h",
                                              "fnet_block_norm_bwd.h")] + [os.path.join(os.path.dirname(HERE), "include", "fluidnet_hip.h")]
 # -packed-fp32-ops: hipcc makes v_pk_{add,mul,fma}_f32 of ordinary float code by itself, and some of their forms have given wrong results on
-# MI355X now and then; the scalar forms are as fast for code that memory bounds.  (The host pass warns that it does not know the feature.)
+# MI355X now and then.  The scalar forms cost what little of the code arithmetic bounds (training step 35.7 -> 35.9 ms, rollout 5818 -> 5758
+# scene-frames/s on one box).  (The host pass warns that it does not know the feature.)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-ffp-contract=off", "-Wall", "-Wno-unused-function", "-Wno-unused-value",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 

@@ -88,7 +88,7 @@ struct RowPlace {
 // wave can be one round ahead of another, never two, so one barrier a round is enough.  All threads of the block call it together.
 template <int L, int N>
 struct RowSum {
-    static constexpr int PITCH = L == 1 ? 4 * 4 : 16;           // places per value: waves of a row times rows of a block
+    static constexpr int PITCH = 16;                            // places per value: waves of a row times rows of a block
     static constexpr int SIZE = L < 8 ? 2 * N * PITCH : 1;
     float* red;
     int turn;

@@ -2,8 +2,9 @@
 
 torch.nn.utils.clip_grad_norm_ as ml/training/trainer.py:192-195 calls it, for the parameters of any module: fp32, bf16 and fp16 gradients
 in one list, dense in any layout or strided views of larger buffers (up to six axes), no elements, odd sizes, any alignment.  (The UNet's own
-parameters lie in one flat buffer; FusedClipAdam clips that inside its step.)  One launch per 240 gradients, of all types, sums the norm, one
-scales; nothing is copied to the host, so both can be captured into a graph.
+parameters lie in one flat buffer; FusedClipAdam clips that inside its step.)  One launch per 240 dense gradients, of all types, sums the norm,
+one scales, and each strided gradient has two of its own (many of them are better packed); nothing is copied to the host, so all can be
+captured into a graph.
 
 Norms are summed in 64 bits in a fixed order: the same gradients give the same bits, and neither a large gradient's square nor the tail of a
 long list is lost.  Clipping multiplies in 32 bits and rounds once.  All gradients must lie on one device (one process per GPU).
@@ -145,8 +146,9 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """Scales the gradients of `parameters` in place by min(1, max_norm / (norm + 1e-6)) and returns the norm that they had (0-dim, fp32, on
     their device).  Parameters without a gradient are passed over.  A norm that is not finite scales as torch does (gradients become 0 or NaN),
-    or raises with error_if_nonfinite=True, which waits for the GPU.  Dense gradients that share memory are refused, and a strided
-    one that appears twice."""
+    or raises with error_if_nonfinite=True, which waits for the GPU.  (Finite gradients whose norm is beyond 32 bits are scaled by the norm as it is,
+    though the value returned is infinite.)  Dense gradients that share memory are refused, and a strided one that appears twice; of strided
+    gradients that overlap otherwise, with each other or with a dense one, the common elements are scaled once for each, as torch does."""
     kind, max_norm = _norm_kind(norm_type), _max_norm(max_norm)
     grads = _grads(parameters)
     if not grads:

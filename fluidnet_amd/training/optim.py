@@ -156,7 +156,9 @@ class ClipAdam:
     Parameters without a gradient are left as they are in a step, moments too; t counts the optimizer's steps.  16-bit parameters have fp32
     masters, made from them at the first step and again when a parameter has been written by something else since the last one (which its
     version counter tells: load_state_dict, in-place operations; after writing through .data call refresh()).  step() can be captured into
-    a graph after one eager step: step count and learning rate are on the device, set param_groups[0]["lr"] and call push_lr() between replays."""
+    a graph after one eager step: step count and learning rate are on the device, set param_groups[0]["lr"] and call push_lr() between replays.  A
+    replay does not look for parameters written by something else: call refresh() after such a write.  One clipping norm, learning rate and
+    weight decay for all parameters: parameter groups are refused."""
 
     def __init__(self, params: Iterable[torch.nn.Parameter], lr: float, max_norm: Optional[float] = 1.0, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 0.0) -> None:
